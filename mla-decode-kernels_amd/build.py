@@ -11,6 +11,7 @@ Products (in-tree, git-ignored, shipped with the source tree):
                              (+ .sources.json: the source hashes it was built
                              from, python/provenance.py)
   lib/gqa_decode_ext*.so     g++: host-only torch operator layer linking the above
+  lib/kv_cache_ext*.so       g++: the same for the cache operators (kv_cache.h)
   lib/libgqa_stream_probe.so hipcc: the streaming-read probe bench.py measures
                              the bandwidth ceiling with (not on the decode path)
   lib/libissue_probe.so      hipcc: MFMA / VALU / LDS issue-rate probes and the
@@ -49,7 +50,8 @@ OBJ_DIR = os.path.join(PKG_DIR, "_build", "obj")  # objects: not shipped to GPU 
 PROBE_LIB = os.path.join(LIB_DIR, "libgqa_stream_probe.so")
 ISSUE_PROBE_LIB = os.path.join(LIB_DIR, "libissue_probe.so")
 HIP_SOURCES = ["gqa_decode_v0.hip", "gqa_decode_split.hip", "gqa_decode_mfma.hip",
-               "gqa_decode_balanced.hip", "mla_decode.hip", "mla_decode_wide.hip"]
+               "gqa_decode_balanced.hip", "mla_decode.hip", "mla_decode_wide.hip",
+               "kv_append.hip", "kv_decode.hip"]
 # Packed fp32 VALU ops are disabled for all device code.
 HIP_FLAGS = [
     f"--offload-arch={ARCH}", "-O3", "-std=c++17", "-fPIC", "-fvisibility=hidden",
@@ -107,11 +109,11 @@ def build_probe(src="stream_probe.hip", lib=PROBE_LIB):
     return lib
 
 
-def ext_filename():
-    return "gqa_decode_ext" + sysconfig.get_config_var("EXT_SUFFIX")
+def ext_filename(name="gqa_decode_ext"):
+    return name + sysconfig.get_config_var("EXT_SUFFIX")
 
 
-def build_extension():
+def build_extension(name="gqa_decode_ext"):
     import torch
     from torch.utils import cpp_extension
 
@@ -121,14 +123,14 @@ def build_extension():
     abi = int(torch._C._GLIBCXX_USE_CXX11_ABI)
     incs = cpp_extension.include_paths() + [INCLUDE, os.path.join(ROCM, "include"),
                                             sysconfig.get_paths()["include"]]
-    out = os.path.join(LIB_DIR, ext_filename())
+    out = os.path.join(LIB_DIR, ext_filename(name))
     tmp = out + ".tmp"
     cmd = [
         "g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-w",
         f"-D_GLIBCXX_USE_CXX11_ABI={abi}", "-DTORCH_API_INCLUDE_EXTENSION_H",
-        "-DTORCH_EXTENSION_NAME=gqa_decode_ext", "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1",
+        f"-DTORCH_EXTENSION_NAME={name}", "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1",
         *[f"-I{i}" for i in incs],
-        os.path.join(PKG_DIR, "python", "gqa_decode_ext.cpp"),
+        os.path.join(PKG_DIR, "python", name + ".cpp"),
         "-o", tmp,
         f"-L{LIB_DIR}", "-lgqa_decode_hip", "-Wl,-rpath,$ORIGIN",
         f"-L{torch_lib}", "-lc10", "-lc10_hip", "-ltorch", "-ltorch_cpu", "-ltorch_python",
@@ -163,6 +165,7 @@ def main(argv=None):
     build_probe("issue_probe.hip", ISSUE_PROBE_LIB)
     if not args.no_ext:
         build_extension()
+        build_extension("kv_cache_ext")
 
 
 if __name__ == "__main__":

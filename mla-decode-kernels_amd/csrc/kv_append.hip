@@ -1,0 +1,443 @@
+// Appends to the paged caches (include/kv_cache.h): norm over each head,
+// position rotation and the store of the new keys and values, in one pass over
+// the step's rows; and the read-back of rows of the 4-bit cache.
+//
+// What bounds them is the bytes: every row is read once and written once, and
+// the arithmetic is a few operations an element. A wave takes four tokens, 16
+// lanes (a DPP row) each, 8 dims a lane, and walks heads: the tokens' places
+// and their angles (16 registers) are found once and serve every head. In
+// the 4-bit cache four tokens of a request, if they are aligned, are one whole
+// 256-byte line of value codes.
+#include "kv_cache.h"
+
+#include "kv_common.hpp"
+
+namespace {
+
+using namespace kv;
+using gqa::dpp_f32;
+using gqa::row16_sum;
+
+constexpr int kWaves = 4;  // waves of a workgroup: neighbouring head ranges of the same tokens
+
+// Columns of the rotation of 8 dims [8i, 8i + 8): y = x c + x' s, x' the pair's
+// other element, the sign of its sine in s.
+struct Turn {
+  float c[8], s[8];
+  int partner;  // the lane (of the wave) that holds x', -1: this one (interleaved pairs)
+  bool on;      // these dims rotate
+};
+
+// kLanes lanes hold a row of 8 kLanes dims, of which the first rot turn.
+template <int kLanes>
+__device__ __forceinline__ Turn load_turn(const float* __restrict__ cos_sin, int rows, int rot,
+                                          int interleaved, int p, int lane) {
+  Turn t;
+  const int i = lane & (kLanes - 1);
+  t.on = 8 * i < rot;
+  t.partner = lane;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) t.c[e] = 1.f, t.s[e] = 0.f;
+  if (!t.on) return t;
+  const int h = rot >> 1;
+  // Column of the first pair of these dims, and the number of pairs in them.
+  const int col = interleaved ? 4 * i : (8 * i < h ? 8 * i : 8 * i - h);
+  if ((uint32_t)p >= (uint32_t)rows) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) t.c[e] = t.s[e] = __builtin_nanf("");
+  } else {
+    const float* row = cos_sin + (size_t)p * rot;
+    if (interleaved) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        t.c[2 * e] = t.c[2 * e + 1] = row[col + e];
+        const float s = row[h + col + e];
+        t.s[2 * e] = -s;
+        t.s[2 * e + 1] = s;
+      }
+    } else {
+      const bool first = 8 * i < h;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        t.c[e] = row[col + e];
+        const float s = row[h + col + e];
+        t.s[e] = first ? -s : s;
+      }
+    }
+  }
+  if (!interleaved) t.partner = 8 * i < h ? lane + (h >> 3) : lane - (h >> 3);
+  return t;
+}
+
+// The pair's other elements of x (every lane of the wave calls this).
+template <class F>
+__device__ __forceinline__ void others(const F (&x)[8], F (&y)[8], const Turn& t, bool interleaved) {
+  if (interleaved) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) y[e] = x[e ^ 1];
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) y[e] = __shfl(x[e], t.partner, 64);
+  }
+}
+
+// Norm over the head's 128 dims (16 lanes), then the rotation.
+__device__ __forceinline__ void norm_turn(float (&x)[8], const float* w, float eps, const Turn& t,
+                                          bool rotate, bool interleaved) {
+  if (w) {
+    float ss = 0.f;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) ss = fmaf(x[e], x[e], ss);
+    const float r = 1.f / sqrtf(row16_sum(ss) * (1.f / kDim) + eps);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) x[e] = x[e] * r * w[e];
+  }
+  if (!rotate) return;
+  float y[8];
+  others(x, y, t, interleaved);
+  if (!t.on) return;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) x[e] = fmaf(x[e], t.c[e], y[e] * t.s[e]);
+}
+
+// The same in fp64, for values whose rounding decides on a 4-bit code: bf16
+// products are exact, the sum of 128 squares nearly, and what is left is off by
+// 2^-50, far less than the chance distance to a border between two codes.
+// (gfx950 runs fp64 FMAs at the rate of fp32 ones.)
+__device__ __forceinline__ void norm_turn64(float (&x)[8], const float* w, float eps,
+                                            const Turn& t, bool rotate, bool interleaved) {
+  double d[8];
+#pragma unroll
+  for (int e = 0; e < 8; ++e) d[e] = x[e];
+  if (w) {
+    double ss = 0.;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) ss = fma(d[e], d[e], ss);
+#pragma unroll
+    for (int o = 1; o < 16; o <<= 1) ss += __shfl_xor(ss, o, 64);
+    const double r = 1. / sqrt(ss * (1. / kDim) + (double)eps);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) d[e] = d[e] * r * (double)w[e];
+  }
+  if (rotate) {
+    double y[8];
+    others(d, y, t, interleaved);
+    if (t.on) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) d[e] = fma(d[e], (double)t.c[e], y[e] * (double)t.s[e]);
+    }
+  }
+#pragma unroll
+  for (int e = 0; e < 8; ++e) x[e] = f32_to_odd(d[e]);
+}
+
+// 8 of a group's 32 values (the other 24 in the quad's other lanes) -> their
+// codes, and the group's scale byte. The scale byte is the biased exponent of the
+// largest magnitude less 2, plus 1 if its significand is over 1.75: magnitudes
+// up to 7 round to 6 or less, those in (7, 8) would be cut to 6, so they take
+// the next scale. v_cvt_scalef32_pk_fp4_f32 divides by the scale (its exponent
+// field alone counts) and rounds to the nearest code, ties to even.
+__device__ __forceinline__ uint32_t encode8(const float (&x)[8], uint32_t& scale) {
+  uint32_t top = 0;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) top = max(top, __float_as_uint(x[e]) & 0x7fffffffu);
+  top = max(top, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)top, 0xB1, 0xF, 0xF, true));
+  top = max(top, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)top, 0x4E, 0xF, 0xF, true));
+  scale = 255u;
+  if (top >= 0x7f800000u) return 0u;
+  const int e = (int)(top >> 23) - 2 + ((top & 0x7fffffu) > 0x600000u ? 1 : 0);
+  scale = (uint32_t)max(e, 1);
+  const float s = __uint_as_float(scale << 23);
+  uint32_t c = 0;
+  c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, x[0], x[1], s, 0);
+  c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, x[2], x[3], s, 1);
+  c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, x[4], x[5], s, 2);
+  c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, x[6], x[7], s, 3);
+  return c;
+}
+
+__device__ __forceinline__ float weight_at(const void* w, int type, int d) {
+  return type == KV_WEIGHT_FP32
+             ? static_cast<const float*>(w)[d]
+             : __uint_as_float((uint32_t) static_cast<const uint16_t*>(w)[d] << 16);
+}
+
+// Grid: x groups of four tokens, y ranges of kWaves * R rows (q heads, then k
+// heads, then v heads); a wave takes R of them.
+template <bool kMx, int R>
+__global__ __launch_bounds__(64 * kWaves) void kv_append_kernel(kv_append_args a, FastDiv bs_div) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int i = lane & 15;
+  const int t = (int)blockIdx.x * 4 + (lane >> 4);
+  const int rows = a.Hq + 2 * a.Hkv;
+  const int r0 = ((int)blockIdx.y * kWaves + wave) * R;
+  if (r0 >= rows) return;
+  const bool in = t < a.T;
+
+  // The rows' loads go out first: they need no place.
+  uint4 raw[R];
+#pragma unroll
+  for (int j = 0; j < R; ++j) {
+    raw[j] = make_uint4(0, 0, 0, 0);
+    const int r = r0 + j;
+    if (!in || r >= rows) continue;
+    const uint16_t* p = r < a.Hq ? a.q + t * a.q_token_stride + r * a.q_head_stride
+                        : r < a.Hq + a.Hkv
+                            ? a.k + t * a.k_token_stride + (r - a.Hq) * a.k_head_stride
+                            : a.v + t * a.v_token_stride + (r - a.Hq - a.Hkv) * a.v_head_stride;
+    raw[j] = load16(p + 8 * i);
+  }
+
+  const Place place = find_place<16>(t, a.T, a.B, a.seq_lens, a.cu_seqlens, lane);
+  int slot;
+  const int block = find_block(place, a.block_table, a.max_blocks, a.num_blocks, bs_div, slot);
+  const bool rotate = a.rotary_dim > 0, inter = a.interleaved != 0;
+  Turn turn{};
+  if (rotate && r0 < a.Hq + a.Hkv)
+    turn = load_turn<16>(a.cos_sin, a.table_rows, a.rotary_dim, a.interleaved,
+                         a.rope_positions && in ? a.rope_positions[t] : place.pos, lane);
+
+#pragma unroll
+  for (int j = 0; j < R; ++j) {
+    const int r = r0 + j;
+    if (r >= rows) break;
+    const bool is_q = r < a.Hq, is_k = !is_q && r < a.Hq + a.Hkv;
+    float x[8];
+    unpack8(raw[j], x);
+    if (is_q || is_k) {
+      const void* wp = is_q ? a.q_weight : a.k_weight;
+      float w[8];
+      if (wp) {
+        const int type = is_q ? a.q_weight_type : a.k_weight_type;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) w[e] = weight_at(wp, type, 8 * i + e);
+      }
+      if (kMx && is_k)
+        norm_turn64(x, wp ? w : nullptr, a.eps, turn, rotate, inter);
+      else
+        norm_turn(x, wp ? w : nullptr, a.eps, turn, rotate, inter);
+    }
+    if (is_q) {
+      if (in)
+        store16(a.q_out + t * a.q_out_token_stride + r * a.q_out_head_stride + 8 * i,
+                place.live ? pack8(x) : make_uint4(0, 0, 0, 0));
+      continue;
+    }
+    const int head = is_k ? r - a.Hq : r - a.Hq - a.Hkv;
+    if constexpr (kMx) {
+      uint32_t scale;
+      const uint32_t code = encode8(x, scale);  // (all lanes: quads exchange maxima)
+      if (block >= 0) {
+        uint8_t* tile = a.mxfp4_cache +
+                        (((size_t)block * a.Hkv + head) * (a.block_size / kTileTokens) +
+                         slot / kTileTokens) * kTileBytes;
+        const int s = slot % kTileTokens;
+        *reinterpret_cast<uint32_t*>(tile + (is_k ? key_code_at(s, i) : value_code_at(s, i))) =
+            code;
+        if ((i & 3) == 0)
+          tile[is_k ? key_scale_at(s, i >> 2) : value_scale_at(s, i >> 2)] = (uint8_t)scale;
+      }
+    } else if (block >= 0) {
+      const size_t at = (((size_t)block * a.block_size + slot) * a.Hkv + head) * kDim + 8 * i;
+      *reinterpret_cast<uint4*>((is_k ? a.k_cache : a.v_cache) + at) = is_k ? pack8(x) : raw[j];
+    }
+  }
+}
+
+// Eight codes of one scale as bf16 (exact: a code has two significant bits).
+__device__ __forceinline__ uint4 decode8(uint32_t code, uint32_t scale) {
+  const float s = __uint_as_float(scale << 23);
+  return make_uint4(
+      __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(code, s, 0)),
+      __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(code, s, 1)),
+      __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(code, s, 2)),
+      __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(code, s, 3)));
+}
+
+// Grid: x groups of four tokens, y groups of kWaves heads.
+__global__ __launch_bounds__(64 * kWaves) void kv_read_mxfp4_kernel(
+    const uint8_t* __restrict__ cache, const int* __restrict__ block_table,
+    const int* __restrict__ seq_lens, const int* __restrict__ cu_seqlens,
+    uint16_t* __restrict__ k_out, uint16_t* __restrict__ v_out, int T, int B, int Hkv,
+    int num_blocks, int block_size, int max_blocks, FastDiv bs_div) {
+  const int lane = threadIdx.x & 63, i = lane & 15;
+  const int t = (int)blockIdx.x * 4 + (lane >> 4);
+  const int head = (int)blockIdx.y * kWaves + (threadIdx.x >> 6);
+  if (head >= Hkv) return;
+  const Place place = find_place<16>(t, T, B, seq_lens, cu_seqlens, lane);
+  if (t >= T) return;
+  int slot;
+  const int block = find_block(place, block_table, max_blocks, num_blocks, bs_div, slot);
+  uint4 k = make_uint4(0, 0, 0, 0), v = k;
+  if (block >= 0) {
+    const uint8_t* tile = cache + (((size_t)block * Hkv + head) * (block_size / kTileTokens) +
+                                   slot / kTileTokens) * kTileBytes;
+    const int s = slot % kTileTokens;
+    k = decode8(*reinterpret_cast<const uint32_t*>(tile + key_code_at(s, i)),
+                tile[key_scale_at(s, i >> 2)]);
+    v = decode8(*reinterpret_cast<const uint32_t*>(tile + value_code_at(s, i)),
+                tile[value_scale_at(s, i >> 2)]);
+  }
+  const size_t at = ((size_t)t * Hkv + head) * kDim + 8 * i;
+  *reinterpret_cast<uint4*>(k_out + at) = k;
+  *reinterpret_cast<uint4*>(v_out + at) = v;
+}
+
+// ------------------------------------------------------------------- MLA
+
+constexpr int kLatent = 512, kRope = 64, kRow = kLatent + kRope;
+
+// A wave takes one token's latent row (pass 0), or eight of its 64-dim rotary
+// rows, 8 lanes each (queries, then the key; passes 1 ..).
+// Grid: x tokens, y groups of kWaves passes.
+__global__ __launch_bounds__(64 * kWaves) void kv_append_mla_kernel(kv_append_mla_args a,
+                                                                    FastDiv bs_div) {
+  const int lane = threadIdx.x & 63;
+  const int t = (int)blockIdx.x;
+  const int pass = (int)blockIdx.y * kWaves + (threadIdx.x >> 6);
+  const int row = (pass - 1) * 8 + (lane >> 3);  // passes 1 ..: q heads, then k_pe
+  const int i = lane & 7;
+  if (pass > (a.h_q + 8) / 8) return;
+  const bool is_q = pass > 0 && row < a.h_q, is_k = pass > 0 && row == a.h_q;
+
+  uint4 raw = make_uint4(0, 0, 0, 0);
+  if (pass == 0)
+    raw = load16(a.c + t * a.c_token_stride + 8 * lane);
+  else if (is_q)
+    raw = load16(a.q_pe + t * a.q_token_stride + row * a.q_head_stride + 8 * i);
+  else if (is_k)
+    raw = load16(a.k_pe + t * a.k_token_stride + 8 * i);
+
+  const Place place = find_place<64>(t, a.T, a.B, a.seq_lens, a.cu_seqlens, lane);
+  int slot;
+  const int block = find_block(place, a.block_table, a.max_blocks, a.num_blocks, bs_div, slot);
+  uint16_t* dst = a.kv_cache + ((size_t)max(block, 0) * a.block_size + slot) * kRow;
+  float x[8];
+  unpack8(raw, x);
+  if (pass == 0) {
+    if (a.c_weight) {
+      float ss = 0.f;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) ss = fmaf(x[e], x[e], ss);
+      const float r = 1.f / sqrtf(gqa::wave_sum(ss) * (1.f / kLatent) + a.eps);
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        x[e] = x[e] * r * weight_at(a.c_weight, a.c_weight_type, 8 * lane + e);
+      raw = pack8(x);
+    }
+    if (block >= 0) *reinterpret_cast<uint4*>(dst + 8 * lane) = raw;
+    return;
+  }
+  const Turn turn = load_turn<8>(a.cos_sin, a.table_rows, kRope, a.interleaved,
+                                 a.rope_positions ? a.rope_positions[t] : place.pos, lane);
+  float y[8];
+  others(x, y, turn, a.interleaved != 0);
+#pragma unroll
+  for (int e = 0; e < 8; ++e) x[e] = fmaf(x[e], turn.c[e], y[e] * turn.s[e]);
+  if (is_q)
+    store16(a.q_out + t * a.q_out_token_stride + row * a.q_out_head_stride + 8 * i,
+            place.live ? pack8(x) : make_uint4(0, 0, 0, 0));
+  else if (is_k && block >= 0)
+    *reinterpret_cast<uint4*>(dst + kLatent + 8 * i) = pack8(x);
+}
+
+// ------------------------------------------------------------------ host
+
+bool bad_weight(const void* w, int type) {
+  return w && type != KV_WEIGHT_BF16 && type != KV_WEIGHT_FP32;
+}
+
+bool misaligned(const void* p, uintptr_t to) { return (reinterpret_cast<uintptr_t>(p) & (to - 1)) != 0; }
+
+// Sizes that every append and read shares.
+hipError_t check_sizes(int T, int B, bool ragged, int num_blocks, int block_size, int max_blocks) {
+  if (T < 0 || T > KV_MAX_TOKENS || B < 0 || num_blocks < 0) return hipErrorInvalidValue;
+  if (block_size < 1 || max_blocks < 1) return hipErrorInvalidValue;
+  if (!ragged && T != B) return hipErrorInvalidValue;
+  return hipSuccess;
+}
+
+hipError_t check_append(const kv_append_args& a, bool mx) {
+  const hipError_t e =
+      check_sizes(a.T, a.B, a.cu_seqlens != nullptr, a.num_blocks, a.block_size, a.max_blocks);
+  if (e != hipSuccess) return e;
+  if (a.Hq < 1 || a.Hkv < 1 || a.Hq > 4096 || a.Hkv > 4096) return hipErrorInvalidValue;
+  if (mx && a.block_size % kTileTokens != 0) return hipErrorInvalidValue;
+  if (a.rotary_dim < 0 || a.rotary_dim > kDim || a.rotary_dim % 16 != 0)
+    return hipErrorInvalidValue;
+  if ((a.rotary_dim > 0) != (a.cos_sin != nullptr) || a.table_rows < 0) return hipErrorInvalidValue;
+  if (bad_weight(a.q_weight, a.q_weight_type) || bad_weight(a.k_weight, a.k_weight_type))
+    return hipErrorInvalidValue;
+  if (a.T == 0) return hipSuccess;
+  if (!a.q || !a.k || !a.v || !a.q_out || !a.block_table || !a.seq_lens)
+    return hipErrorInvalidValue;
+  if (a.num_blocks > 0) {
+    if (mx ? (!a.mxfp4_cache || misaligned(a.mxfp4_cache, 4))
+           : (!a.k_cache || !a.v_cache || misaligned(a.k_cache, 16) || misaligned(a.v_cache, 16)))
+      return hipErrorInvalidValue;
+  }
+  return hipSuccess;
+}
+
+template <bool kMx>
+int append(const kv_append_args* args, hipStream_t stream) {
+  if (!args) return hipErrorInvalidValue;
+  const hipError_t e = check_append(*args, kMx);
+  if (e != hipSuccess) return e;
+  if (args->T == 0) return hipSuccess;
+  const kv_append_args a = *args;
+  const int rows = a.Hq + 2 * a.Hkv;
+  const unsigned tokens = (unsigned)((a.T + 3) / 4);
+  const auto grid = [&](int R) { return dim3(tokens, (rows + kWaves * R - 1) / (kWaves * R)); };
+  if ((int64_t)tokens * rows <= 16384)
+    kv_append_kernel<kMx, 1><<<grid(1), 64 * kWaves, 0, stream>>>(a, make_fastdiv(a.block_size));
+  else
+    kv_append_kernel<kMx, 4><<<grid(4), 64 * kWaves, 0, stream>>>(a, make_fastdiv(a.block_size));
+  return hipGetLastError();
+}
+
+}  // namespace
+
+extern "C" int kv_append_launch(const kv_append_args* args, hipStream_t stream) {
+  return append<false>(args, stream);
+}
+
+extern "C" int kv_append_mxfp4_launch(const kv_append_args* args, hipStream_t stream) {
+  return append<true>(args, stream);
+}
+
+extern "C" int kv_read_mxfp4_launch(const uint8_t* mxfp4_cache, const int* block_table,
+                                    const int* seq_lens, const int* cu_seqlens, uint16_t* k_out,
+                                    uint16_t* v_out, int T, int B, int Hkv, int num_blocks,
+                                    int block_size, int max_blocks, hipStream_t stream) {
+  const hipError_t e = check_sizes(T, B, cu_seqlens != nullptr, num_blocks, block_size, max_blocks);
+  if (e != hipSuccess) return e;
+  if (Hkv < 1 || Hkv > 4096 || block_size % kTileTokens != 0) return hipErrorInvalidValue;
+  if (T == 0) return hipSuccess;
+  if (!block_table || !seq_lens || !k_out || !v_out || misaligned(k_out, 16) ||
+      misaligned(v_out, 16) || (num_blocks > 0 && (!mxfp4_cache || misaligned(mxfp4_cache, 4))))
+    return hipErrorInvalidValue;
+  kv_read_mxfp4_kernel<<<dim3((unsigned)((T + 3) / 4), (Hkv + kWaves - 1) / kWaves), 64 * kWaves, 0,
+                         stream>>>(mxfp4_cache, block_table, seq_lens, cu_seqlens, k_out, v_out, T,
+                                   B, Hkv, num_blocks, block_size, max_blocks,
+                                   make_fastdiv(block_size));
+  return hipGetLastError();
+}
+
+extern "C" int kv_append_mla_launch(const kv_append_mla_args* args, hipStream_t stream) {
+  if (!args) return hipErrorInvalidValue;
+  const kv_append_mla_args a = *args;
+  const hipError_t e =
+      check_sizes(a.T, a.B, a.cu_seqlens != nullptr, a.num_blocks, a.block_size, a.max_blocks);
+  if (e != hipSuccess) return e;
+  if (a.h_q < 1 || a.h_q > 4096 || a.table_rows < 0 || bad_weight(a.c_weight, a.c_weight_type))
+    return hipErrorInvalidValue;
+  if (a.T == 0) return hipSuccess;
+  if (!a.q_pe || !a.c || !a.k_pe || !a.q_out || !a.block_table || !a.seq_lens || !a.cos_sin ||
+      (a.num_blocks > 0 && (!a.kv_cache || misaligned(a.kv_cache, 16))))
+    return hipErrorInvalidValue;
+  const int passes = 1 + (a.h_q + 8) / 8;  // the latent row, then h_q + 1 rotary rows
+  kv_append_mla_kernel<<<dim3((unsigned)a.T, (passes + kWaves - 1) / kWaves), 64 * kWaves, 0,
+                         stream>>>(a, make_fastdiv(a.block_size));
+  return hipGetLastError();
+}

@@ -1,0 +1,123 @@
+// Layout of the 4-bit paged cache (include/kv_cache.h) and the device helpers
+// its kernels and the append kernels share.
+#pragma once
+
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+#include "gqa_device.hpp"
+#include "kv_places.hpp"
+
+namespace kv {
+
+using gqa::bf16_hi;
+using gqa::bf16_lo;
+using gqa::f32_to_bf16_bits;
+using gqa::FastDiv;
+using gqa::fastdiv;
+using gqa::make_fastdiv;
+
+constexpr int kDim = 128;
+constexpr int kTileTokens = 16;
+constexpr int kTileBytes = 2176;
+constexpr int kValueCodes = 1024;   // byte offsets in a tile
+constexpr int kKeyScales = 2048;
+constexpr int kValueScales = 2112;
+
+// Byte offsets of a token's share of a tile: r the token in the tile, i the
+// group of 8 dims (codes: 4 bytes), g the group of 32 dims (scale: 1 byte).
+__host__ __device__ constexpr int key_code_at(int r, int i) {
+  return (i >> 2) * 256 + r * 16 + (i & 3) * 4;
+}
+__host__ __device__ constexpr int value_code_at(int r, int i) {
+  return kValueCodes + (r >> 2) * 256 + i * 16 + (r & 3) * 4;
+}
+__host__ __device__ constexpr int key_scale_at(int r, int g) { return kKeyScales + g * 16 + r; }
+__host__ __device__ constexpr int value_scale_at(int r, int g) {
+  return kValueScales + (r >> 2) * 16 + g * 4 + (r & 3);
+}
+static_assert(key_code_at(15, 15) + 4 == kValueCodes && value_code_at(15, 15) + 4 == kKeyScales &&
+                  key_scale_at(15, 3) + 1 == kValueScales && value_scale_at(15, 3) + 1 == kTileBytes,
+              "the four parts fill a tile");
+
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef __bf16 bf16x2_t __attribute__((ext_vector_type(2)));
+
+// 16 bytes at an address that is a multiple of 2 (rows of strided views can
+// start anywhere; gfx950 loads and stores them whole at any alignment).
+typedef u32x4 u32x4_any __attribute__((aligned(2)));
+__device__ __forceinline__ uint4 load16(const uint16_t* p) {
+  const u32x4 v = *reinterpret_cast<const u32x4_any*>(p);
+  return make_uint4(v.x, v.y, v.z, v.w);
+}
+__device__ __forceinline__ void store16(uint16_t* p, const uint4& v) {
+  *reinterpret_cast<u32x4_any*>(p) = u32x4{v.x, v.y, v.z, v.w};
+}
+
+__device__ __forceinline__ void unpack8(const uint4& w, float (&x)[8]) {
+  x[0] = bf16_lo(w.x); x[1] = bf16_hi(w.x); x[2] = bf16_lo(w.y); x[3] = bf16_hi(w.y);
+  x[4] = bf16_lo(w.z); x[5] = bf16_hi(w.z); x[6] = bf16_lo(w.w); x[7] = bf16_hi(w.w);
+}
+// Round to nearest even, once: the only rounding of a bf16 append.
+__device__ __forceinline__ uint4 pack8(const float (&x)[8]) {
+  uint32_t w[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    w[i] = f32_to_bf16_bits(x[2 * i]) | (f32_to_bf16_bits(x[2 * i + 1]) << 16);
+  return make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+// fp64 -> fp32 rounded to odd: truncated, with the last bit set if anything was
+// cut off. A later rounding to fewer than 23 bits then gives what rounding the
+// fp64 value itself would have given (no double rounding).
+__device__ __forceinline__ float f32_to_odd(double d) {
+  const float f = (float)d;
+  const double back = (double)f;
+  uint32_t u = __float_as_uint(f);
+  if (back != d && d == d) {
+    if (__builtin_fabs(back) > __builtin_fabs(d)) --u;  // rounded up (from infinity too)
+    u |= 1u;
+  }
+  return __uint_as_float(u);
+}
+
+// The place of row t of the new tokens (kv_cache.h), computed by each group of
+// kGroup lanes (a power of two, aligned) for its own t; 0 <= t. Every lane of the
+// wave calls it.
+template <int kGroup>
+__device__ __forceinline__ Place find_place(int t, int T, int B, const int* __restrict__ seq_lens,
+                                            const int* __restrict__ cu_seqlens, int lane) {
+  int b = t, first = t, next = t + 1;
+  if (cu_seqlens) {
+    const int sub = lane & (kGroup - 1), shift = lane & ~(kGroup - 1);
+    Search s = Search::begin(B);
+    // Groups may need different numbers of steps: all lanes stay until all are
+    // done (the ballot is the wave's).
+    while (__builtin_amdgcn_ballot_w64(!s.done())) {
+      const int step = s.step(kGroup), at = s.lo + sub * step;
+      const bool under = at < s.hi && cu_seqlens[at] <= t;
+      uint64_t m = __builtin_amdgcn_ballot_w64(under) >> shift;
+      if constexpr (kGroup < 64) m &= (uint64_t(1) << (kGroup & 63)) - 1;
+      s.narrow(step, __popcll(m));
+    }
+    b = s.request();
+    if (b < B) first = cu_seqlens[b], next = cu_seqlens[b + 1];
+  }
+  if (b >= B || t >= T) return Place{0, 0, false};
+  return place_in(t, b, first, next, seq_lens[b]);
+}
+
+// The block id of a position, or -1 where the cache has no place for it.
+__device__ __forceinline__ int find_block(const Place& p, const int* __restrict__ block_table,
+                                          int max_blocks, int num_blocks, const FastDiv& bs_div,
+                                          int& slot) {
+  slot = 0;
+  if (!p.live) return -1;
+  const uint32_t lb = fastdiv((uint32_t)p.pos, bs_div);
+  slot = p.pos - (int)(lb * bs_div.d);
+  if (lb >= (uint32_t)max_blocks) return -1;
+  const int id = block_table[(size_t)p.b * max_blocks + lb];
+  return (uint32_t)id < (uint32_t)num_blocks ? id : -1;
+}
+
+}  // namespace kv

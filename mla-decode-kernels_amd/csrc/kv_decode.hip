@@ -1,0 +1,750 @@
+// Single-token GQA decode over the 4-bit paged cache (include/kv_cache.h).
+//
+// One wave streams a piece of one (request, kv-head): units of 32 tokens, two
+// 16-token tiles of the cache, which the lanes load whole (16 bytes of key codes
+// and of value codes a lane and tile) and already in the matrix cores' operand
+// layouts. A unit, with lane l = (c, g) = (l % 16, l / 16):
+//
+//   QK^T   S[16 tok x 16 cols] = K . Q^T on v_mfma_scale_f32_16x16x128_f8f6f4:
+//          A = the key codes as they lie in the cache (lane: token c, dims
+//          32g .. +32) with their scale bytes, B = the queries in two e4m3
+//          parts, q = 2^E (hi + lo / 16) with one E a head: a bf16 value has 8
+//          significant bits and e4m3 has 4, so the parts hold every value down
+//          to 2^-13 of the head's largest exactly, and the rest to 2^-21 of it.
+//          Groups of up to 8 q-heads put the hi parts into columns 0-7 and the
+//          lo parts into columns 8-15 of one instruction; wider ones take two.
+//   softmax on the C layout: lane (c, g) holds tokens 4g .. 4g+3 of each tile
+//          for column c.
+//   PV     O^T[128 dims x 16 cols] += V^T . P^T on 8 v_mfma_f32_16x16x32_bf16,
+//          contraction slot (g, e): token 4g+e of the first tile, 4g+e-4 of the
+//          second, which is where the scores lie (no data crosses lanes) and
+//          what a lane loads of the values: 8 dims 8c .. 8c+7 of those 8
+//          tokens. v_cvt_scalef32_pk_bf16_fp4 widens them exactly, scale and
+//          all. P enters as two bf16 parts as well, p = p_hi + p_lo (truncated:
+//          2^-15 relative), in columns 0-7 and 8-15 or in two products.
+//          The sum of the weights is one more product, with ones for V^T, so
+//          that the weights that are summed are those that were multiplied.
+//
+// Work is shared out evenly whatever the lengths: all units of the batch in
+// (request, kv-head, token) order, an equal run of them to each workgroup and
+// within it to each wave. A wave finishes the segments that lie in its run;
+// its cut pieces meet in LDS, those that the workgroup's run cuts in the
+// workspace, where a second kernel folds them in order.
+#include <math.h>
+
+#include <algorithm>
+#include <type_traits>
+
+#include "gqa_launch.hpp"
+#include "kv_cache.h"
+#include "kv_common.hpp"
+
+namespace {
+
+using namespace kv;
+using gqa::dpp_f32;
+using gqa::exp2_fast;
+using gqa::kNegInf;
+using gqa::wave_max;
+using gqa::xor16_max;
+using gqa::xor32_max;
+
+typedef __bf16 bf16x8_t __attribute__((ext_vector_type(8)));
+typedef float f32x2_t __attribute__((ext_vector_type(2)));
+typedef float f32x4_t __attribute__((ext_vector_type(4)));
+typedef int i32x8_t __attribute__((ext_vector_type(8)));
+
+constexpr int kUnit = 32;       // tokens a wave takes at a time
+constexpr int kWaves = 8;       // waves of a workgroup
+constexpr int kThreads = 64 * kWaves;
+constexpr int kPitch = 132;     // floats of a head's state: acc [128], m, l, pad
+constexpr int kMinUnits = 2;    // units a wave gets before another workgroup joins in
+
+constexpr int kHasA = 1, kEndsA = 2, kHasZ = 4;  // pieces of a share (Record::flags)
+
+struct Record {
+  int flags, seg_a, seg_z, pad;
+};
+
+struct DecodeArgs {
+  const uint16_t* q;
+  const uint8_t* cache;
+  const int* block_table;
+  const int* seq_lens;
+  uint16_t* out;
+  float* states;     // [workgroups][2][heads][kPitch]
+  Record* records;   // [workgroups]
+  int B, Hq, Hkv, G, chunks, heads;  // heads: the largest number of q-heads of a segment
+  int num_blocks, tiles_per_block, max_blocks, capacity;
+  FastDiv tile_div;  // by tiles_per_block
+  float scale;       // |scale| log2(e)
+  float sign;        // of scale
+  int per_segment;   // a workgroup for each segment: no shares, nothing in the workspace
+};
+
+// A unit's data in registers.
+struct Unit {
+  uint4 k[2], v[2];
+  uint32_t ks[2], vs[2];
+};
+
+template <bool kWide>
+struct State {
+  float m;         // running maximum of the column's raw scores
+  f32x4_t o[8];    // o[j][e]: dim 32g + 8e + j of column c
+  f32x4_t l;       // sum of the weights (four times the same)
+};
+
+template <bool kWide>
+struct Query {
+  i32x8_t part[kWide ? 2 : 1];
+  int scale[kWide ? 2 : 1];
+};
+
+// The queries of heads h0 .. h0 + nh - 1 of request b as the B operand: lane
+// (c, g), bytes 0-15: dims 16g .., bytes 16-31: dims 64 + 16g ...
+template <bool kWide>
+__device__ __forceinline__ Query<kWide> load_query(const DecodeArgs& a, int b, int h0, int nh,
+                                                   int c, int g) {
+  const int head = kWide ? c : (c & 7);
+  float x[32];
+#pragma unroll
+  for (int part = 0; part < 4; ++part) {
+    uint4 w = make_uint4(0, 0, 0, 0);
+    if (head < nh)
+      w = *reinterpret_cast<const uint4*>(a.q + ((size_t)b * a.Hq + h0 + head) * kDim +
+                                          (part >> 1) * 64 + 16 * g + 8 * (part & 1));
+    float y[8];
+    unpack8(w, y);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) x[8 * part + e] = y[e] * a.sign;
+  }
+  float top = 0.f;
+#pragma unroll
+  for (int e = 0; e < 32; ++e) top = fmaxf(top, fabsf(x[e]));
+  top = xor32_max(xor16_max(top));
+  // E puts the largest magnitude into [128, 256); e4m3 ends at 448.
+  const int E = top > 0.f ? max((int)(__float_as_uint(top) >> 23) - 127 - 7, -118) : 0;
+  const float up = __uint_as_float((uint32_t)(127 - E) << 23);
+  Query<kWide> q;
+  uint32_t hi[8], lo[8];
+#pragma unroll
+  for (int w = 0; w < 8; ++w) {
+    int h = 0, r = 0;
+    const float y0 = x[4 * w] * up, y1 = x[4 * w + 1] * up;
+    const float y2 = x[4 * w + 2] * up, y3 = x[4 * w + 3] * up;
+    h = __builtin_amdgcn_cvt_pk_fp8_f32(y0, y1, h, false);
+    h = __builtin_amdgcn_cvt_pk_fp8_f32(y2, y3, h, true);
+    const f32x2_t b0 = __builtin_amdgcn_cvt_pk_f32_fp8(h, false);
+    const f32x2_t b1 = __builtin_amdgcn_cvt_pk_f32_fp8(h, true);
+    r = __builtin_amdgcn_cvt_pk_fp8_f32((y0 - b0[0]) * 16.f, (y1 - b0[1]) * 16.f, r, false);
+    r = __builtin_amdgcn_cvt_pk_fp8_f32((y2 - b1[0]) * 16.f, (y3 - b1[1]) * 16.f, r, true);
+    hi[w] = (uint32_t)h;
+    lo[w] = (uint32_t)r;
+  }
+  if constexpr (kWide) {
+#pragma unroll
+    for (int w = 0; w < 8; ++w) {
+      q.part[0][w] = (int)hi[w];
+      q.part[1][w] = (int)lo[w];
+    }
+    q.scale[0] = E + 127;
+    q.scale[1] = E + 123;
+  } else {
+    const bool low = c >= 8;
+#pragma unroll
+    for (int w = 0; w < 8; ++w) q.part[0][w] = (int)(low ? lo[w] : hi[w]);
+    q.scale[0] = E + (low ? 123 : 127);
+  }
+  return q;
+}
+
+// Where a unit's two tiles lie, and which of its tokens count.
+struct Spot {
+  const uint8_t* tile[2];
+  int valid[2];  // tokens of each tile that count (0 .. 16)
+};
+
+// Block ids through the constant address space: scalar loads, which do not
+// share a counter with the tiles' loads (as gqa_scan_mfma.hpp measured).
+typedef const __attribute__((address_space(4))) int* const_ints;
+
+__device__ __forceinline__ Spot find_unit(const DecodeArgs& a, const_ints table, int head, int len,
+                                          int u) {
+  Spot s;
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    const int first = u * kUnit + h * kTileTokens;
+    s.valid[h] = min(max(len - first, 0), kTileTokens);
+    s.tile[h] = h ? s.tile[0] : a.cache;
+    if (s.valid[h] == 0) continue;  // past the end: any tile that may be read
+    const uint32_t t = (uint32_t)first / kTileTokens;
+    const uint32_t lb = fastdiv(t, a.tile_div);
+    const int id = table[lb];
+    if ((uint32_t)id >= (uint32_t)a.num_blocks) {
+      s.valid[h] = 0;
+      continue;
+    }
+    s.tile[h] = a.cache + (((size_t)id * a.Hkv + head) * a.tiles_per_block +
+                           (t - lb * a.tile_div.d)) * kTileBytes;
+  }
+  return s;
+}
+
+__device__ __forceinline__ uint4 stream16(const uint8_t* p) {
+  const u32x4 v = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(p));
+  return make_uint4(v.x, v.y, v.z, v.w);
+}
+
+__device__ __forceinline__ void load_unit(const Spot& s, int lane, Unit& u) {
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    const uint8_t* p = s.tile[h];
+    u.k[h] = stream16(p + 16 * lane);
+    u.v[h] = stream16(p + kValueCodes + 16 * lane);
+    u.ks[h] = p[kKeyScales + lane];
+    u.vs[h] = *reinterpret_cast<const uint32_t*>(p + kValueScales + (lane >> 4) * 16 +
+                                                 ((lane & 15) >> 2) * 4);
+  }
+}
+
+// Fold a unit into the state. kMask: some of its tokens do not count.
+template <bool kWide, bool kMask>
+__device__ __forceinline__ void fold_unit(const Unit& u, const int (&valid)[2],
+                                          const Query<kWide>& q, float scale, int c, int g,
+                                          State<kWide>& st) {
+  float s[8];
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    const i32x8_t k = {(int)u.k[h].x, (int)u.k[h].y, (int)u.k[h].z, (int)u.k[h].w, 0, 0, 0, 0};
+    f32x4_t d = {0.f, 0.f, 0.f, 0.f};
+    d = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(k, q.part[0], d, 4, 0, 0, (int)u.ks[h], 0,
+                                                         q.scale[0]);
+    if constexpr (kWide)
+      d = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(k, q.part[1], d, 4, 0, 0,
+                                                           (int)u.ks[h], 0, q.scale[1]);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      // Columns c and c + 8 hold the two parts: a rotation by 8 within the row.
+      s[4 * h + e] = kWide ? d[e] : d[e] + dpp_f32<0x128>(d[e]);
+      if (kMask && 4 * g + e >= valid[h]) s[4 * h + e] = kNegInf;
+    }
+  }
+  float mx = s[0];
+#pragma unroll
+  for (int e = 1; e < 8; ++e) mx = fmaxf(mx, s[e]);
+  mx = xor32_max(xor16_max(mx));
+  if (__builtin_amdgcn_ballot_w64(mx > st.m)) {
+    const float mn = fmaxf(st.m, mx);
+    const float alpha = mn == kNegInf ? 1.f : exp2_fast((st.m - mn) * scale);
+    st.m = mn;
+    st.l *= alpha;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) st.o[j] *= alpha;
+  }
+  const float ms = kMask && st.m == kNegInf ? 0.f : st.m * scale;
+  uint32_t p[kWide ? 2 : 1][8];
+  const uint32_t low = kWide || c < 8 ? 0u : 0xffff0000u;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    float w = exp2_fast(fmaf(s[e], scale, -ms));
+    if (kMask && s[e] == kNegInf) w = 0.f;
+    const uint32_t bits = __float_as_uint(w);
+    if constexpr (kWide) {
+      p[0][e] = bits;
+      p[1][e] = __float_as_uint(w - __uint_as_float(bits & 0xffff0000u));
+    } else {
+      p[0][e] = __float_as_uint(w - __uint_as_float(bits & low));
+    }
+  }
+  constexpr uint32_t kLow16 = 0x05040100u, kHigh16 = 0x07060302u;
+  bf16x8_t pb[kWide ? 2 : 1];
+#pragma unroll
+  for (int i = 0; i < (kWide ? 2 : 1); ++i) {
+    u32x4 w;
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      w[e] = __builtin_amdgcn_perm(p[i][2 * e + 1], p[i][2 * e], kHigh16);
+    pb[i] = __builtin_bit_cast(bf16x8_t, w);
+  }
+  // Scale bytes to exponent fields; the bits around them do not count.
+  float vs[8];
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    vs[4 * h + 0] = __uint_as_float(u.vs[h] << 23);
+    vs[4 * h + 1] = __uint_as_float(u.vs[h] << 15);
+    vs[4 * h + 2] = __uint_as_float(u.vs[h] << 7);
+    vs[4 * h + 3] = __uint_as_float(u.vs[h] >> 1);
+    if constexpr (kMask) {  // what lies behind the last token may be anything
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (4 * g + e >= valid[h]) vs[4 * h + e] = 1.f;
+    }
+  }
+  const uint32_t code[8] = {u.v[0].x, u.v[0].y, u.v[0].z, u.v[0].w,
+                            u.v[1].x, u.v[1].y, u.v[1].z, u.v[1].w};
+  const auto pairs = [&](auto byte, u32x4& even, u32x4& odd) {
+    uint32_t d[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+      d[e] = __builtin_bit_cast(
+          uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(code[e], vs[e], decltype(byte)::value));
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      even[e] = __builtin_amdgcn_perm(d[2 * e + 1], d[2 * e], kLow16);
+      odd[e] = __builtin_amdgcn_perm(d[2 * e + 1], d[2 * e], kHigh16);
+    }
+  };
+  const auto two_dims = [&](auto byte) {
+    constexpr int j = 2 * decltype(byte)::value;
+    u32x4 even, odd;
+    pairs(byte, even, odd);
+#pragma unroll
+    for (int i = 0; i < (kWide ? 2 : 1); ++i) {
+      st.o[j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, even), pb[i],
+                                                        st.o[j], 0, 0, 0);
+      st.o[j + 1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, odd),
+                                                            pb[i], st.o[j + 1], 0, 0, 0);
+    }
+  };
+  const u32x4 one = {0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u};
+#pragma unroll
+  for (int i = 0; i < (kWide ? 2 : 1); ++i)
+    st.l = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, one), pb[i], st.l, 0,
+                                                   0, 0);
+  two_dims(std::integral_constant<int, 0>{});
+  two_dims(std::integral_constant<int, 1>{});
+  two_dims(std::integral_constant<int, 2>{});
+  two_dims(std::integral_constant<int, 3>{});
+}
+
+// Units [u0, u1) of a segment. The next unit's loads go out before a unit is
+// folded.
+template <bool kWide>
+__device__ __forceinline__ void scan_piece(const DecodeArgs& a, const_ints table, int head, int len,
+                                           int u0, int u1, const Query<kWide>& q, int lane,
+                                           State<kWide>& st) {
+  const int c = lane & 15, g = lane >> 4;
+  st.m = kNegInf;
+  st.l = f32x4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int j = 0; j < 8; ++j) st.o[j] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+  const auto fold = [&](const Unit& u, const Spot& s) {
+    if (s.valid[0] + s.valid[1] == kUnit)
+      fold_unit<kWide, false>(u, s.valid, q, a.scale, c, g, st);
+    else
+      fold_unit<kWide, true>(u, s.valid, q, a.scale, c, g, st);
+  };
+  Unit x0, x1;
+  Spot s0 = find_unit(a, table, head, len, u0), s1;
+  load_unit(s0, lane, x0);
+  s1 = find_unit(a, table, head, len, min(u0 + 1, u1 - 1));
+  int u = u0;
+  while (true) {
+    // Past the end the last unit is loaded once more, and not folded.
+    load_unit(s1, lane, x1);
+    const Spot s2 = find_unit(a, table, head, len, min(u + 2, u1 - 1));
+    fold(x0, s0);
+    if (++u >= u1) break;
+    load_unit(s2, lane, x0);
+    s0 = s2;
+    const Spot s3 = find_unit(a, table, head, len, min(u + 2, u1 - 1));
+    fold(x1, s1);
+    s1 = s3;
+    if (++u >= u1) break;
+  }
+}
+
+// out = acc / l; a segment without a single token gets zeros.
+__device__ __forceinline__ float normal(float acc, float l) { return l == 0.f ? 0.f : acc / l; }
+
+__device__ __forceinline__ int segment_heads(const DecodeArgs& a, int seg, int& b, int& hc, int& h0) {
+  const int Hc = a.Hkv * a.chunks;
+  b = seg / Hc;
+  hc = seg - b * Hc;
+  const int kv_head = hc / a.chunks, first = (hc - kv_head * a.chunks) * 16;
+  h0 = kv_head * a.G + first;
+  return min(16, a.G - first);
+}
+
+__device__ __forceinline__ int length_of(const DecodeArgs& a, int b) {
+  return min(max(((const_ints)a.seq_lens)[b], 0), a.capacity);
+}
+__device__ __forceinline__ int units_of(int len) { return (int)(((uint32_t)len + kUnit - 1) / kUnit); }
+
+template <bool kWide>
+__global__ __launch_bounds__(kThreads, 2) void kv_decode_kernel(DecodeArgs a) {
+  extern __shared__ float slots[];  // [kWaves][2][heads][kPitch]
+  __shared__ uint32_t prefix[kThreads];
+  __shared__ uint32_t wave_total[kWaves];
+  __shared__ Record meta[kWaves];
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int c = lane & 15, g = lane >> 4;
+  const int Hc = a.Hkv * a.chunks;
+  const int wg = blockIdx.x, nwg = gridDim.x;
+
+  // Requests without tokens get zeros.
+  for (int b = a.per_segment ? wg / Hc : wg; b < a.B; b += a.per_segment ? a.B : nwg) {
+    if (length_of(a, b) > 0) continue;
+    for (int i = tid; i < a.Hq * kDim / 8; i += kThreads)
+      reinterpret_cast<uint4*>(a.out + (size_t)b * a.Hq * kDim)[i] = make_uint4(0, 0, 0, 0);
+  }
+
+  // This wave's run of units: it starts at unit u of segment (b, hc) and holds n.
+  int b, hc, u, len;
+  uint64_t n;
+  if (a.per_segment) {
+    b = wg / Hc;
+    hc = wg - b * Hc;
+    len = length_of(a, b);
+    const uint32_t total = (uint32_t)units_of(len);
+    u = (int)(total * (uint64_t)wave / kWaves);
+    n = total * (uint64_t)(wave + 1) / kWaves - u;
+  } else {
+    // Prefix sums of the requests' units, a slice of them to each thread.
+    const int slice = (a.B + kThreads - 1) / kThreads;
+    uint32_t sum = 0;
+    for (int i = 0; i < slice; ++i) {
+      const int r = tid * slice + i;
+      if (r < a.B) sum += (uint32_t)units_of(min(max(a.seq_lens[r], 0), a.capacity));
+    }
+    uint32_t inc = sum;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+      const uint32_t y = __shfl_up(inc, o, 64);
+      if (lane >= o) inc += y;
+    }
+    if (lane == 63) wave_total[wave] = inc;
+    __syncthreads();
+    uint32_t base = 0, total = 0;
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) {
+      const uint32_t y = wave_total[w];
+      if (w < wave) base += y;
+      total += y;
+    }
+    prefix[tid] = base + inc - sum;
+    __syncthreads();
+    const uint64_t all = (uint64_t)total * Hc;
+    // Few units: as many workgroups as give their waves kMinUnits each.
+    const uint64_t want = (all + kWaves * kMinUnits - 1) / (kWaves * kMinUnits);
+    const uint64_t used = want < (uint64_t)nwg ? (want ? want : 1) : (uint64_t)nwg;
+    uint64_t w0 = 0, w1 = 0;
+    if ((uint64_t)wg < used) {
+      w0 = all * (uint64_t)wg / used;
+      w1 = all * (uint64_t)(wg + 1) / used;
+    }
+    const uint64_t p0 = w0 + (w1 - w0) * wave / kWaves, p1 = w0 + (w1 - w0) * (wave + 1) / kWaves;
+    n = p1 - p0;
+    b = hc = u = len = 0;
+    if (n > 0) {
+      // The slice that holds unit x, then the request in it.
+      const uint32_t x = (uint32_t)(p0 / Hc);
+      int found = 0;
+#pragma unroll
+      for (int i = 0; i < kWaves; ++i)
+        found += __popcll(__builtin_amdgcn_ballot_w64(prefix[i * 64 + lane] <= x));
+      const int at = __builtin_amdgcn_readfirstlane(found - 1);
+      uint32_t pre = __builtin_amdgcn_readfirstlane(prefix[at]);
+      b = at * slice;
+      len = length_of(a, b);
+      while (x - pre >= (uint32_t)units_of(len)) {
+        pre += (uint32_t)units_of(len);
+        len = length_of(a, ++b);
+      }
+      const uint64_t rem = p0 - (uint64_t)pre * Hc;
+      hc = (int)(rem / (uint32_t)units_of(len));
+      u = (int)(rem - (uint64_t)hc * units_of(len));
+    }
+  }
+
+  int flags = 0, seg_a = 0, seg_z = 0;
+  const size_t slot_floats = (size_t)a.heads * kPitch;
+  while (n > 0) {
+    const int units = units_of(len);
+    const int u1 = (int)min((uint64_t)units, u + n);
+    const int kv_head = hc / a.chunks, first = (hc - kv_head * a.chunks) * 16;
+    const int h0 = kv_head * a.G + first, nh = min(16, a.G - first);
+    const Query<kWide> q = load_query<kWide>(a, b, h0, nh, c, g);
+    State<kWide> st;
+    scan_piece<kWide>(a, (const_ints)(a.block_table + (size_t)b * a.max_blocks), kv_head, len, u,
+                      u1, q, lane, st);
+    if constexpr (!kWide) {
+      st.l += f32x4_t{dpp_f32<0x128>(st.l[0]), 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) st.o[j][e] += dpp_f32<0x128>(st.o[j][e]);
+    }
+    const float l = st.l[0];
+    if (u == 0 && u1 == units) {
+      if (c < nh) {
+        uint16_t* dst = a.out + ((size_t)b * a.Hq + h0 + c) * kDim + 32 * g;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          float y[8];
+#pragma unroll
+          for (int j = 0; j < 8; ++j) y[j] = normal(st.o[j][e], l);
+          *reinterpret_cast<uint4*>(dst + 8 * e) = pack8(y);
+        }
+      }
+    } else {
+      const int which = u > 0 ? 0 : 1;
+      if (which == 0) {
+        flags |= kHasA | (u1 == units ? kEndsA : 0);
+        seg_a = b * Hc + hc;
+      } else {
+        flags |= kHasZ;
+        seg_z = b * Hc + hc;
+      }
+      if (c < nh) {
+        float* dst = slots + (wave * 2 + which) * slot_floats + c * kPitch;
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+#pragma unroll
+          for (int j = 0; j < 8; j += 4)
+            *reinterpret_cast<f32x4_t*>(dst + 32 * g + 8 * e + j) =
+                f32x4_t{st.o[j][e], st.o[j + 1][e], st.o[j + 2][e], st.o[j + 3][e]};
+        if (g == 0) {
+          dst[kDim] = st.m == kNegInf ? kNegInf : st.m * a.scale;
+          dst[kDim + 1] = l;
+        }
+      }
+    }
+    n -= (uint64_t)(u1 - u);
+    if (n == 0) break;
+    u = 0;
+    if (++hc == Hc) {
+      hc = 0;
+      do len = length_of(a, ++b);
+      while (len == 0);
+    }
+  }
+  if (lane == 0) meta[wave] = Record{flags, seg_a, seg_z, 0};
+  __syncthreads();
+
+  // The pieces of a segment cut between waves are neighbours: a run starts
+  // at a wave's second piece (Z), or at the first piece of all if the workgroup's
+  // run starts inside a segment, and takes the first pieces (A) of the waves
+  // after it up to the segment's end. A wave folds heads wave, wave + kWaves, ..
+  // of every run, two dims a lane.
+  Record rec{0, 0, 0, 0};
+  for (int start = -1; start < kWaves; ++start) {
+    int seg, w, which;
+    bool ends = false;
+    if (start < 0) {
+      for (w = 0; w < kWaves && meta[w].flags == 0; ++w) {
+      }
+      // (Waves in front without a cut piece are empty: had they held whole
+      // segments, this one would start at a segment's start.)
+      if (w == kWaves || !(meta[w].flags & kHasA)) continue;
+      seg = meta[w].seg_a;
+      which = 0;
+    } else {
+      if (!(meta[start].flags & kHasZ)) continue;
+      w = start;
+      seg = meta[w].seg_z;
+      which = 1;
+    }
+    seg = __builtin_amdgcn_readfirstlane(seg);
+    // The run's pieces: bit 2 w + which.
+    uint32_t pieces = 1u << (2 * w + which);
+    if (which == 0 && (meta[w].flags & kEndsA)) ends = true;
+    for (++w; w < kWaves && !ends; ++w) {
+      if (!(meta[w].flags & kHasA)) continue;
+      pieces |= 1u << (2 * w);
+      ends = (meta[w].flags & kEndsA) != 0;
+    }
+    pieces = __builtin_amdgcn_readfirstlane(pieces);
+    const bool to_out = start >= 0 && ends;
+    if (start < 0) {
+      rec.flags |= kHasA | (ends ? kEndsA : 0);
+      rec.seg_a = seg;
+    } else if (!ends) {
+      rec.flags |= kHasZ;
+      rec.seg_z = seg;
+    }
+    int sb, shc, h0;
+    const int nh = segment_heads(a, seg, sb, shc, h0);
+    for (int h = wave; h < nh; h += kWaves) {
+      float M = kNegInf;
+      for (uint32_t left = pieces; left; left &= left - 1)
+        M = fmaxf(M, slots[__builtin_ctz(left) * slot_floats + h * kPitch + kDim]);
+      float L = 0.f, x = 0.f, y = 0.f;
+      for (uint32_t left = pieces; left; left &= left - 1) {
+        const float* p = slots + __builtin_ctz(left) * slot_floats + h * kPitch;
+        const float f = M == kNegInf ? 0.f : exp2_fast(p[kDim] - M);
+        L = fmaf(p[kDim + 1], f, L);
+        x = fmaf(p[2 * lane], f, x);
+        y = fmaf(p[2 * lane + 1], f, y);
+      }
+      if (to_out) {
+        reinterpret_cast<uint32_t*>(a.out + ((size_t)sb * a.Hq + h0 + h) * kDim)[lane] =
+            f32_to_bf16_bits(normal(x, L)) | (f32_to_bf16_bits(normal(y, L)) << 16);
+      } else {
+        float* dst = a.states + ((size_t)wg * 2 + (start < 0 ? 0 : 1)) * slot_floats + h * kPitch;
+        reinterpret_cast<float2*>(dst)[lane] = make_float2(x, y);
+        if (lane == 0) reinterpret_cast<float2*>(dst + kDim)[0] = make_float2(M, L);
+      }
+    }
+  }
+  if (!a.per_segment && tid == 0) a.records[wg] = rec;
+}
+
+// Segments cut between workgroups: the workgroup whose first piece ends one
+// folds it, from the one whose last piece starts it. A wave to each head; pieces in
+// share order, 8 at a time.
+constexpr int kMergeWaves = 4;
+__global__ __launch_bounds__(64 * kMergeWaves) void kv_decode_merge_kernel(DecodeArgs a) {
+  const int wg = blockIdx.x, lane = threadIdx.x & 63;
+  const Record rec = a.records[wg];
+  if ((rec.flags & (kHasA | kEndsA)) != (kHasA | kEndsA)) return;
+  int from = -1;
+  for (int base = wg - 1; base >= 0 && from < 0; base -= 64) {
+    const int w = base - lane;
+    const uint64_t hit =
+        __builtin_amdgcn_ballot_w64(w >= 0 && (a.records[max(w, 0)].flags & kHasZ) != 0);
+    if (hit) from = base - (int)__builtin_ctzll(hit);
+  }
+  if (from < 0) return;
+  int b, hc, h0;
+  const int nh = segment_heads(a, rec.seg_a, b, hc, h0);
+  const int h = (int)blockIdx.y * kMergeWaves + (threadIdx.x >> 6);
+  if (h >= nh) return;
+  const size_t slot_floats = (size_t)a.heads * kPitch;
+  // Workgroups without a share between the first and the last have no piece;
+  // there are none (shares go to the first workgroups), so every one counts.
+  const auto state = [&](int w) {
+    return a.states + ((size_t)w * 2 + (w == from ? 1 : 0)) * slot_floats + h * kPitch;
+  };
+  float mloc = kNegInf;
+  for (int w = from + lane; w <= wg; w += 64) mloc = fmaxf(mloc, state(w)[kDim]);
+  const float M = wave_max(mloc);
+  float L = 0.f, x = 0.f, y = 0.f;
+  constexpr int kBatch = 8;
+  for (int w0 = from; w0 <= wg; w0 += kBatch) {
+    float2 v[kBatch], ml[kBatch];
+#pragma unroll
+    for (int i = 0; i < kBatch; ++i) {
+      const float* p = state(min(w0 + i, wg));
+      v[i] = reinterpret_cast<const float2*>(p)[lane];
+      ml[i] = *reinterpret_cast<const float2*>(p + kDim);
+    }
+#pragma unroll
+    for (int i = 0; i < kBatch; ++i) {
+      if (w0 + i > wg) break;
+      const float f = M == kNegInf ? 0.f : exp2_fast(ml[i].x - M);
+      L = fmaf(ml[i].y, f, L);
+      x = fmaf(v[i].x, f, x);
+      y = fmaf(v[i].y, f, y);
+    }
+  }
+  reinterpret_cast<uint32_t*>(a.out + ((size_t)b * a.Hq + h0 + h) * kDim)[lane] =
+      f32_to_bf16_bits(normal(x, L)) | (f32_to_bf16_bits(normal(y, L)) << 16);
+}
+
+struct Shape {
+  int G, chunks, heads, capacity, workgroups;
+  bool per_segment;
+};
+
+// Longest sequence, in units, that a workgroup takes alone.
+constexpr int kAloneUnits = 4 * kWaves;
+
+bool shape_of(int B, int Hq, int Hkv, int num_blocks, int block_size, int max_blocks,
+              int num_workgroups, Shape& s) {
+  if (B < 0 || B > (1 << 20) || Hq < 1 || Hkv < 1 || Hq > 4096 || Hq % Hkv != 0) return false;
+  if (num_blocks < 0 || block_size < 1 || block_size % kTileTokens != 0 || max_blocks < 1)
+    return false;
+  const int64_t cap = num_blocks == 0 ? 0 : (int64_t)block_size * max_blocks;
+  // Token positions and the batch's units fit 31 bits.
+  if (cap > INT32_MAX - kUnit || (int64_t)B * ((cap + kUnit - 1) / kUnit) > INT32_MAX) return false;
+  if ((int64_t)B * Hq > (int64_t(1) << 28)) return false;
+  s.G = Hq / Hkv;
+  s.chunks = (s.G + 15) / 16;
+  s.heads = std::min(s.G, 16);
+  s.capacity = (int)cap;
+  s.per_segment = num_workgroups <= 0 && (cap + kUnit - 1) / kUnit <= kAloneUnits;
+  s.workgroups = num_workgroups;
+  if (s.per_segment)
+    s.workgroups = B * Hkv * s.chunks;
+  else if (num_workgroups <= 0)
+    s.workgroups = gqa::device_cu_count();
+  return s.workgroups <= (1 << 22);
+}
+
+size_t workspace_bytes(const Shape& s) {
+  if (s.per_segment) return 0;
+  return (size_t)s.workgroups * (sizeof(Record) + 2 * (size_t)s.heads * kPitch * sizeof(float));
+}
+
+}  // namespace
+
+extern "C" size_t kv_decode_mxfp4_workspace_bytes(int B, int Hq, int Hkv, int block_size,
+                                                  int max_blocks, int num_workgroups) {
+  Shape s;
+  if (!shape_of(B, Hq, Hkv, 1, block_size, max_blocks, num_workgroups, s) || s.workgroups < 1)
+    return 0;
+  return workspace_bytes(s);
+}
+
+extern "C" int kv_decode_mxfp4_launch(const uint16_t* q, const uint8_t* mxfp4_cache,
+                                      const int* block_table, const int* seq_lens, uint16_t* out,
+                                      int B, int Hq, int Hkv, int num_blocks, int block_size,
+                                      int max_blocks, float scale, int num_workgroups,
+                                      void* workspace, size_t workspace_bytes_, hipStream_t stream) {
+  Shape s;
+  if (!shape_of(B, Hq, Hkv, num_blocks, block_size, max_blocks, num_workgroups, s))
+    return hipErrorInvalidValue;
+  if (!isfinite(scale)) return hipErrorInvalidValue;
+  if (B == 0) return hipSuccess;
+  if (s.workgroups < 1) return hipErrorInvalidValue;
+  const auto bad = [](const void* p, uintptr_t to) {
+    return !p || (reinterpret_cast<uintptr_t>(p) & (to - 1)) != 0;
+  };
+  if (bad(q, 16) || bad(out, 16) || !block_table || !seq_lens ||
+      (num_blocks > 0 && bad(mxfp4_cache, 16)))
+    return hipErrorInvalidValue;
+  const size_t need = workspace_bytes(s);
+  if (need > 0 && (bad(workspace, 16) || workspace_bytes_ < need)) return hipErrorInvalidValue;
+  DecodeArgs a{};
+  a.q = q;
+  a.cache = mxfp4_cache;
+  a.block_table = block_table;
+  a.seq_lens = seq_lens;
+  a.out = out;
+  a.records = static_cast<Record*>(workspace);
+  a.states = need ? reinterpret_cast<float*>(static_cast<char*>(workspace) +
+                                             sizeof(Record) * s.workgroups)
+                  : nullptr;
+  a.B = B;
+  a.Hq = Hq;
+  a.Hkv = Hkv;
+  a.G = s.G;
+  a.chunks = s.chunks;
+  a.heads = s.heads;
+  a.num_blocks = num_blocks;
+  a.tiles_per_block = block_size / kTileTokens;
+  a.max_blocks = max_blocks;
+  a.capacity = s.capacity;
+  a.tile_div = make_fastdiv((uint32_t)a.tiles_per_block);
+  // (A scale of 0 weighs all tokens alike; the smallest normal does as well and
+  // keeps 0 * infinity out of the kernel.)
+  a.scale = std::max(fabsf(scale) * gqa::kLog2e, 1.17549435e-38f);
+  a.sign = scale < 0.f ? -1.f : 1.f;
+  a.per_segment = s.per_segment;
+  const size_t lds = (size_t)kWaves * 2 * s.heads * kPitch * sizeof(float);
+  const auto kernel = s.G > 8 ? kv_decode_kernel<true> : kv_decode_kernel<false>;
+  if (lds > 65536) {  // more than the default share of a CU's 160 KiB
+    const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel),
+                                             hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
+    if (e != hipSuccess) return e;
+  }
+  kernel<<<s.workgroups, kThreads, lds, stream>>>(a);
+  hipError_t e = hipGetLastError();
+  if (e != hipSuccess || s.per_segment) return e;
+  kv_decode_merge_kernel<<<dim3(s.workgroups, (s.heads + kMergeWaves - 1) / kMergeWaves),
+                           64 * kMergeWaves, 0, stream>>>(a);
+  return hipGetLastError();
+}

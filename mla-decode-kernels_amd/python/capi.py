@@ -15,6 +15,7 @@ _PKG_DIR = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 LIB_PATH = os.path.join(_PKG_DIR, "lib", "libgqa_decode_hip.so")
 HEADER_PATH = os.path.join(os.path.dirname(_PKG_DIR), "include", "gqa_decode.h")
 MLA_HEADER_PATH = os.path.join(os.path.dirname(_PKG_DIR), "include", "mla_decode.h")
+KV_HEADER_PATH = os.path.join(os.path.dirname(_PKG_DIR), "include", "kv_cache.h")
 
 HIP_SUCCESS = 0
 HIP_ERROR_INVALID_VALUE = 1
@@ -22,6 +23,35 @@ HIP_ERROR_INVALID_VALUE = 1
 _vp = ctypes.c_void_p
 _i = ctypes.c_int
 _LAUNCH_ARGS = [_vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, ctypes.c_float]
+
+
+
+class KvAppendArgs(ctypes.Structure):
+    """kv_append_args of include/kv_cache.h."""
+    _fields_ = ([(n, _vp) for n in ("q", "k", "v", "q_out")]
+                + [(f"{n}_{s}_stride", ctypes.c_int64) for n in ("q", "k", "v", "q_out")
+                   for s in ("token", "head")]
+                + [(n, _vp) for n in ("k_cache", "v_cache", "mxfp4_cache", "block_table",
+                                      "seq_lens", "cu_seqlens", "rope_positions", "cos_sin",
+                                      "q_weight", "k_weight")]
+                + [(n, _i) for n in ("q_weight_type", "k_weight_type", "T", "B", "Hq", "Hkv",
+                                     "num_blocks", "block_size", "max_blocks", "table_rows",
+                                     "rotary_dim", "interleaved")]
+                + [("eps", ctypes.c_float)])
+
+
+class KvAppendMlaArgs(ctypes.Structure):
+    """kv_append_mla_args of include/kv_cache.h."""
+    _fields_ = ([(n, _vp) for n in ("q_pe", "c", "k_pe", "q_out")]
+                + [(n, ctypes.c_int64) for n in ("q_token_stride", "q_head_stride",
+                                                 "c_token_stride", "k_token_stride",
+                                                 "q_out_token_stride", "q_out_head_stride")]
+                + [(n, _vp) for n in ("kv_cache", "block_table", "seq_lens", "cu_seqlens",
+                                      "rope_positions", "cos_sin", "c_weight")]
+                + [(n, _i) for n in ("c_weight_type", "T", "B", "h_q", "num_blocks", "block_size",
+                                     "max_blocks", "table_rows", "interleaved")]
+                + [("eps", ctypes.c_float)])
+
 
 _lib = None
 
@@ -38,6 +68,11 @@ def declared_functions(header=None, prefix="gqa_decode_"):
 def declared_mla_functions():
     """Names of the functions include/mla_decode.h declares."""
     return declared_functions(MLA_HEADER_PATH, "mla_decode_")
+
+
+def declared_kv_functions():
+    """Names of the functions include/kv_cache.h declares."""
+    return declared_functions(KV_HEADER_PATH, "kv_")
 
 
 def lib():
@@ -104,6 +139,20 @@ def bind(path):
     L.mla_decode_workspace_bytes.restype = ctypes.c_size_t
     L.mla_decode_pick_num_splits.argtypes = [_i] * 6
     L.mla_decode_pick_num_splits.restype = _i
+    if hasattr(L, "kv_append_launch"):
+        for name, args in (("kv_append_launch", KvAppendArgs),
+                           ("kv_append_mxfp4_launch", KvAppendArgs),
+                           ("kv_append_mla_launch", KvAppendMlaArgs)):
+            fn = getattr(L, name)
+            fn.argtypes = [ctypes.POINTER(args), _vp]
+            fn.restype = _i
+        L.kv_read_mxfp4_launch.argtypes = [_vp] * 6 + [_i] * 6 + [_vp]
+        L.kv_read_mxfp4_launch.restype = _i
+        L.kv_decode_mxfp4_launch.argtypes = ([_vp] * 5 + [_i] * 6
+                                             + [ctypes.c_float, _i, _vp, ctypes.c_size_t, _vp])
+        L.kv_decode_mxfp4_launch.restype = _i
+        L.kv_decode_mxfp4_workspace_bytes.argtypes = [_i] * 6
+        L.kv_decode_mxfp4_workspace_bytes.restype = ctypes.c_size_t
     return L
 
 
@@ -203,6 +252,33 @@ def balanced_launch_noalloc(*args):
     """gqa_decode_balanced_launch_noalloc: the balanced launch on the library's
     own per-device scratch array (no workspace argument)."""
     return lib().gqa_decode_balanced_launch_noalloc(*args)
+
+
+def kv_append_launch(args, stream):
+    """kv_append_launch; args a KvAppendArgs."""
+    return lib().kv_append_launch(ctypes.byref(args), stream)
+
+
+def kv_append_mxfp4_launch(args, stream):
+    return lib().kv_append_mxfp4_launch(ctypes.byref(args), stream)
+
+
+def kv_append_mla_launch(args, stream):
+    """kv_append_mla_launch; args a KvAppendMlaArgs."""
+    return lib().kv_append_mla_launch(ctypes.byref(args), stream)
+
+
+def kv_read_mxfp4_launch(*args):
+    return lib().kv_read_mxfp4_launch(*args)
+
+
+def kv_decode_mxfp4_launch(*args):
+    return lib().kv_decode_mxfp4_launch(*args)
+
+
+def kv_decode_mxfp4_workspace_bytes(B, Hq, Hkv, block_size, max_blocks, num_workgroups):
+    return lib().kv_decode_mxfp4_workspace_bytes(B, Hq, Hkv, block_size, max_blocks,
+                                                 num_workgroups)
 
 
 # GQA_DECODE_NOALLOC_SCRATCH_BYTES in include/gqa_decode.h.
