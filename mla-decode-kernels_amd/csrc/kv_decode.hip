@@ -77,6 +77,7 @@ struct DecodeArgs {
   int B, Hq, Hkv, G, chunks, heads;  // heads: the largest number of q-heads of a segment
   int num_blocks, tiles_per_block, max_blocks, capacity;
   FastDiv tile_div;  // by tiles_per_block
+  FastDiv head_div;  // by Hkv * chunks
   float scale;       // |scale| log2(e)
   float sign;        // of scale
   int per_segment;   // a workgroup for each segment: no shares, nothing in the workspace
@@ -360,7 +361,7 @@ __device__ __forceinline__ float normal(float acc, float l) { return l == 0.f ? 
 
 __device__ __forceinline__ int segment_heads(const DecodeArgs& a, int seg, int& b, int& hc, int& h0) {
   const int Hc = a.Hkv * a.chunks;
-  b = seg / Hc;
+  b = (int)fastdiv((uint32_t)seg, a.head_div);
   hc = seg - b * Hc;
   const int kv_head = hc / a.chunks, first = (hc - kv_head * a.chunks) * 16;
   h0 = kv_head * a.G + first;
@@ -371,6 +372,24 @@ __device__ __forceinline__ int length_of(const DecodeArgs& a, int b) {
   return min(max(((const_ints)a.seq_lens)[b], 0), a.capacity);
 }
 __device__ __forceinline__ int units_of(int len) { return (int)(((uint32_t)len + kUnit - 1) / kUnit); }
+
+// Sums over the lanes up to this one (of values whose total fits 32 bits): within
+// each row of 16 by DPP shifts, then the rows' totals.
+template <int kShift>
+__device__ __forceinline__ uint32_t add_shifted(uint32_t x) {
+  return x + (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x110 + kShift, 0xF, 0xF, true);
+}
+__device__ __forceinline__ uint32_t wave_prefix(uint32_t x) {
+  x = add_shifted<1>(x);
+  x = add_shifted<2>(x);
+  x = add_shifted<4>(x);
+  x = add_shifted<8>(x);
+  const int lane = threadIdx.x & 63;
+  const uint32_t r0 = (uint32_t)__builtin_amdgcn_readlane((int)x, 15);
+  const uint32_t r1 = (uint32_t)__builtin_amdgcn_readlane((int)x, 31);
+  const uint32_t r2 = (uint32_t)__builtin_amdgcn_readlane((int)x, 47);
+  return x + (lane >= 16 ? r0 : 0) + (lane >= 32 ? r1 : 0) + (lane >= 48 ? r2 : 0);
+}
 
 template <bool kWide>
 __global__ __launch_bounds__(kThreads, 2) void kv_decode_kernel(DecodeArgs a) {
@@ -385,7 +404,7 @@ __global__ __launch_bounds__(kThreads, 2) void kv_decode_kernel(DecodeArgs a) {
   const int wg = blockIdx.x, nwg = gridDim.x;
 
   // Requests without tokens get zeros.
-  for (int b = a.per_segment ? wg / Hc : wg; b < a.B; b += a.per_segment ? a.B : nwg) {
+  for (int b = a.per_segment ? (int)fastdiv((uint32_t)wg, a.head_div) : wg; b < a.B; b += a.per_segment ? a.B : nwg) {
     if (length_of(a, b) > 0) continue;
     for (int i = tid; i < a.Hq * kDim / 8; i += kThreads)
       reinterpret_cast<uint4*>(a.out + (size_t)b * a.Hq * kDim)[i] = make_uint4(0, 0, 0, 0);
@@ -393,69 +412,75 @@ __global__ __launch_bounds__(kThreads, 2) void kv_decode_kernel(DecodeArgs a) {
 
   // This wave's run of units: it starts at unit u of segment (b, hc) and holds n.
   int b, hc, u, len;
-  uint64_t n;
+  uint32_t n;
   if (a.per_segment) {
-    b = wg / Hc;
+    b = (int)fastdiv((uint32_t)wg, a.head_div);
     hc = wg - b * Hc;
     len = length_of(a, b);
     const uint32_t total = (uint32_t)units_of(len);
-    u = (int)(total * (uint64_t)wave / kWaves);
-    n = total * (uint64_t)(wave + 1) / kWaves - u;
+    u = (int)(total * (uint32_t)wave / kWaves);
+    n = total * (uint32_t)(wave + 1) / kWaves - u;
   } else {
-    // Prefix sums of the requests' units, a slice of them to each thread.
-    const int slice = (a.B + kThreads - 1) / kThreads;
+    // Prefix sums of the requests' units, a slice of them to each lane of one
+    // wave (every wave for itself), or to each thread of the workgroup.
+    const bool small = a.B <= 64;
+    const int slice = small ? 1 : (a.B + kThreads - 1) / kThreads;
+    const int mine = small ? lane : tid;
     uint32_t sum = 0;
     for (int i = 0; i < slice; ++i) {
-      const int r = tid * slice + i;
+      const int r = mine * slice + i;
       if (r < a.B) sum += (uint32_t)units_of(min(max(a.seq_lens[r], 0), a.capacity));
     }
-    uint32_t inc = sum;
+    const uint32_t inc = wave_prefix(sum);
+    uint32_t base = 0, total = (uint32_t)__builtin_amdgcn_readlane((int)inc, 63);
+    if (!small) {
+      if (lane == 63) wave_total[wave] = inc;
+      __syncthreads();
+      total = 0;
 #pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-      const uint32_t y = __shfl_up(inc, o, 64);
-      if (lane >= o) inc += y;
+      for (int w = 0; w < kWaves; ++w) {
+        const uint32_t y = wave_total[w];
+        if (w < wave) base += y;
+        total += y;
+      }
+      prefix[tid] = base + inc - sum;
+      __syncthreads();
+      total = (uint32_t)__builtin_amdgcn_readfirstlane((int)total);
     }
-    if (lane == 63) wave_total[wave] = inc;
-    __syncthreads();
-    uint32_t base = 0, total = 0;
-#pragma unroll
-    for (int w = 0; w < kWaves; ++w) {
-      const uint32_t y = wave_total[w];
-      if (w < wave) base += y;
-      total += y;
-    }
-    prefix[tid] = base + inc - sum;
-    __syncthreads();
-    const uint64_t all = (uint64_t)total * Hc;
+    const uint32_t all = total * (uint32_t)Hc;
     // Few units: as many workgroups as give their waves kMinUnits each.
-    const uint64_t want = (all + kWaves * kMinUnits - 1) / (kWaves * kMinUnits);
-    const uint64_t used = want < (uint64_t)nwg ? (want ? want : 1) : (uint64_t)nwg;
-    uint64_t w0 = 0, w1 = 0;
-    if ((uint64_t)wg < used) {
-      w0 = all * (uint64_t)wg / used;
-      w1 = all * (uint64_t)(wg + 1) / used;
-    }
-    const uint64_t p0 = w0 + (w1 - w0) * wave / kWaves, p1 = w0 + (w1 - w0) * (wave + 1) / kWaves;
-    n = p1 - p0;
+    const uint32_t want = max(1u, (all + kWaves * kMinUnits - 1) / (kWaves * kMinUnits));
+    const uint32_t used = min(want, (uint32_t)nwg);
+    const uint32_t each = all / used, more = all - each * used;
+    const uint32_t w0 = (uint32_t)wg * each + min((uint32_t)wg, more);
+    const uint32_t share = (uint32_t)wg < used ? each + ((uint32_t)wg < more ? 1 : 0) : 0;
+    const uint32_t p0 = w0 + (uint32_t)((uint64_t)share * wave / kWaves);
+    n = w0 + (uint32_t)((uint64_t)share * (wave + 1) / kWaves) - p0;
     b = hc = u = len = 0;
     if (n > 0) {
       // The slice that holds unit x, then the request in it.
-      const uint32_t x = (uint32_t)(p0 / Hc);
+      const uint32_t x = fastdiv(p0, a.head_div);
       int found = 0;
+      uint32_t pre;
+      if (small) {
+        const uint32_t mine_before = inc - sum;
+        found = __popcll(__builtin_amdgcn_ballot_w64(mine_before <= x));
+        pre = (uint32_t)__builtin_amdgcn_readlane((int)mine_before, found - 1);
+      } else {
 #pragma unroll
-      for (int i = 0; i < kWaves; ++i)
-        found += __popcll(__builtin_amdgcn_ballot_w64(prefix[i * 64 + lane] <= x));
-      const int at = __builtin_amdgcn_readfirstlane(found - 1);
-      uint32_t pre = __builtin_amdgcn_readfirstlane(prefix[at]);
-      b = at * slice;
+        for (int i = 0; i < kWaves; ++i)
+          found += __popcll(__builtin_amdgcn_ballot_w64(prefix[i * 64 + lane] <= x));
+        pre = (uint32_t)__builtin_amdgcn_readfirstlane((int)prefix[found - 1]);
+      }
+      b = __builtin_amdgcn_readfirstlane((found - 1) * slice);
       len = length_of(a, b);
       while (x - pre >= (uint32_t)units_of(len)) {
         pre += (uint32_t)units_of(len);
         len = length_of(a, ++b);
       }
-      const uint64_t rem = p0 - (uint64_t)pre * Hc;
-      hc = (int)(rem / (uint32_t)units_of(len));
-      u = (int)(rem - (uint64_t)hc * units_of(len));
+      const uint32_t rem = p0 - pre * (uint32_t)Hc, units = (uint32_t)units_of(len);
+      hc = (int)(rem / units);
+      u = (int)(rem - (uint32_t)hc * units);
     }
   }
 
@@ -463,7 +488,7 @@ __global__ __launch_bounds__(kThreads, 2) void kv_decode_kernel(DecodeArgs a) {
   const size_t slot_floats = (size_t)a.heads * kPitch;
   while (n > 0) {
     const int units = units_of(len);
-    const int u1 = (int)min((uint64_t)units, u + n);
+    const int u1 = (int)min((uint32_t)units, u + n);
     const int kv_head = hc / a.chunks, first = (hc - kv_head * a.chunks) * 16;
     const int h0 = kv_head * a.G + first, nh = min(16, a.G - first);
     const Query<kWide> q = load_query<kWide>(a, b, h0, nh, c, g);
@@ -512,7 +537,7 @@ __global__ __launch_bounds__(kThreads, 2) void kv_decode_kernel(DecodeArgs a) {
         }
       }
     }
-    n -= (uint64_t)(u1 - u);
+    n -= (uint32_t)(u1 - u);
     if (n == 0) break;
     u = 0;
     if (++hc == Hc) {
@@ -527,38 +552,25 @@ __global__ __launch_bounds__(kThreads, 2) void kv_decode_kernel(DecodeArgs a) {
   // The pieces of a segment cut between waves are neighbours: a run starts
   // at a wave's second piece (Z), or at the first piece of all if the workgroup's
   // run starts inside a segment, and takes the first pieces (A) of the waves
-  // after it up to the segment's end. A wave folds heads wave, wave + kWaves, ..
-  // of every run, two dims a lane.
+  // after it up to the segment's end. Each head of each run is one wave's, two
+  // dims a lane. Bit w of the masks is wave w's.
+  const Record m = meta[lane & (kWaves - 1)];
+  const auto bits = [&](int flag) {
+    return (uint32_t)__builtin_amdgcn_ballot_w64((m.flags & flag) != 0) & ((1u << kWaves) - 1);
+  };
+  const uint32_t has_a = bits(kHasA), ends_a = bits(kEndsA), has_z = bits(kHasZ);
   Record rec{0, 0, 0, 0};
-  for (int start = -1; start < kWaves; ++start) {
-    int seg, w, which;
-    bool ends = false;
-    if (start < 0) {
-      for (w = 0; w < kWaves && meta[w].flags == 0; ++w) {
-      }
-      // (Waves in front without a cut piece are empty: had they held whole
-      // segments, this one would start at a segment's start.)
-      if (w == kWaves || !(meta[w].flags & kHasA)) continue;
-      seg = meta[w].seg_a;
-      which = 0;
-    } else {
-      if (!(meta[start].flags & kHasZ)) continue;
-      w = start;
-      seg = meta[w].seg_z;
-      which = 1;
-    }
-    seg = __builtin_amdgcn_readfirstlane(seg);
-    // The run's pieces: bit 2 w + which.
-    uint32_t pieces = 1u << (2 * w + which);
-    if (which == 0 && (meta[w].flags & kEndsA)) ends = true;
-    for (++w; w < kWaves && !ends; ++w) {
-      if (!(meta[w].flags & kHasA)) continue;
-      pieces |= 1u << (2 * w);
-      ends = (meta[w].flags & kEndsA) != 0;
-    }
-    pieces = __builtin_amdgcn_readfirstlane(pieces);
-    const bool to_out = start >= 0 && ends;
-    if (start < 0) {
+  int turn = 0;  // heads handed out so far
+  const auto fold_run = [&](int w, int which) {
+    // From wave w's piece on: A pieces up to the first that ends its segment.
+    const uint32_t behind = which ? ~((2u << w) - 1) : ~((1u << w) - 1);
+    const uint32_t last = ends_a & behind;
+    const bool ends = last != 0;
+    const uint32_t upto = ends ? (last & -last) * 2 - 1 : ~0u;
+    const uint32_t as = has_a & behind & upto;  // waves whose A pieces belong to it
+    const int seg = __builtin_amdgcn_readlane(which ? m.seg_z : m.seg_a, w);
+    const bool to_out = which && ends;
+    if (!which) {
       rec.flags |= kHasA | (ends ? kEndsA : 0);
       rec.seg_a = seg;
     } else if (!ends) {
@@ -567,77 +579,112 @@ __global__ __launch_bounds__(kThreads, 2) void kv_decode_kernel(DecodeArgs a) {
     }
     int sb, shc, h0;
     const int nh = segment_heads(a, seg, sb, shc, h0);
-    for (int h = wave; h < nh; h += kWaves) {
+    int h = (wave - turn) & (kWaves - 1);
+    turn += nh;
+    for (; h < nh; h += kWaves) {
+      // Piece i: wave i's A, or piece kWaves: the Z that starts the run.
+      const auto piece = [&](int i) {
+        return slots + (i == kWaves ? w * 2 + 1 : i * 2) * slot_floats + h * kPitch;
+      };
+      const uint32_t live = as | (which ? 1u << kWaves : 0u);
+      float2 ml[kWaves + 1], v[kWaves + 1];
       float M = kNegInf;
-      for (uint32_t left = pieces; left; left &= left - 1)
-        M = fmaxf(M, slots[__builtin_ctz(left) * slot_floats + h * kPitch + kDim]);
+#pragma unroll
+      for (int i = 0; i <= kWaves; ++i) {
+        if (!(live >> i & 1)) continue;
+        ml[i] = *reinterpret_cast<const float2*>(piece(i) + kDim);
+        v[i] = reinterpret_cast<const float2*>(piece(i))[lane];
+      }
+#pragma unroll
+      for (int i = 0; i <= kWaves; ++i)
+        if (live >> i & 1) M = fmaxf(M, ml[i].x);
       float L = 0.f, x = 0.f, y = 0.f;
-      for (uint32_t left = pieces; left; left &= left - 1) {
-        const float* p = slots + __builtin_ctz(left) * slot_floats + h * kPitch;
-        const float f = M == kNegInf ? 0.f : exp2_fast(p[kDim] - M);
-        L = fmaf(p[kDim + 1], f, L);
-        x = fmaf(p[2 * lane], f, x);
-        y = fmaf(p[2 * lane + 1], f, y);
+#pragma unroll
+      for (int j = 0; j <= kWaves; ++j) {
+        const int i = j ? j - 1 : kWaves;  // in the order of the tokens
+        if (!(live >> i & 1)) continue;
+        const float f = M == kNegInf ? 0.f : exp2_fast(ml[i].x - M);
+        L = fmaf(ml[i].y, f, L);
+        x = fmaf(v[i].x, f, x);
+        y = fmaf(v[i].y, f, y);
       }
       if (to_out) {
         reinterpret_cast<uint32_t*>(a.out + ((size_t)sb * a.Hq + h0 + h) * kDim)[lane] =
             f32_to_bf16_bits(normal(x, L)) | (f32_to_bf16_bits(normal(y, L)) << 16);
       } else {
-        float* dst = a.states + ((size_t)wg * 2 + (start < 0 ? 0 : 1)) * slot_floats + h * kPitch;
+        float* dst = a.states + ((size_t)wg * 2 + which) * slot_floats + h * kPitch;
         reinterpret_cast<float2*>(dst)[lane] = make_float2(x, y);
         if (lane == 0) reinterpret_cast<float2*>(dst + kDim)[0] = make_float2(M, L);
       }
     }
+  };
+  // (A first wave with a cut piece that has no A piece starts at a segment's
+  // start, as those in front of it then did, empty or not.)
+  const uint32_t any = has_a | has_z;
+  if (any) {
+    const int first = __builtin_ctz(any);
+    if (has_a >> first & 1) fold_run(first, 0);
+    for (uint32_t left = has_z; left; left &= left - 1) fold_run(__builtin_ctz(left), 1);
   }
   if (!a.per_segment && tid == 0) a.records[wg] = rec;
 }
 
 // Segments cut between workgroups: the workgroup whose first piece ends one
 // folds it, from the one whose last piece starts it. A wave to each head; pieces in
-// share order, 8 at a time.
+// share order.
 constexpr int kMergeWaves = 4;
 __global__ __launch_bounds__(64 * kMergeWaves) void kv_decode_merge_kernel(DecodeArgs a) {
   const int wg = blockIdx.x, lane = threadIdx.x & 63;
-  const Record rec = a.records[wg];
-  if ((rec.flags & (kHasA | kEndsA)) != (kHasA | kEndsA)) return;
+  // Lane i reads record wg - i: the workgroup's own, and those in front.
+  Record r = a.records[max(wg - lane, 0)];
+  const int flags = __builtin_amdgcn_readfirstlane(r.flags);
+  const int seg = __builtin_amdgcn_readfirstlane(r.seg_a);
+  if ((flags & (kHasA | kEndsA)) != (kHasA | kEndsA)) return;
   int from = -1;
-  for (int base = wg - 1; base >= 0 && from < 0; base -= 64) {
-    const int w = base - lane;
-    const uint64_t hit =
-        __builtin_amdgcn_ballot_w64(w >= 0 && (a.records[max(w, 0)].flags & kHasZ) != 0);
-    if (hit) from = base - (int)__builtin_ctzll(hit);
+  uint64_t hit = __builtin_amdgcn_ballot_w64(lane > 0 && lane <= wg && (r.flags & kHasZ) != 0);
+  for (int base = wg;; hit = __builtin_amdgcn_ballot_w64(
+                           lane <= base && (a.records[max(base - lane, 0)].flags & kHasZ) != 0)) {
+    if (hit) {
+      from = base - (int)__builtin_ctzll(hit);
+      break;
+    }
+    base -= 64;
+    if (base < 0) return;
   }
-  if (from < 0) return;
   int b, hc, h0;
-  const int nh = segment_heads(a, rec.seg_a, b, hc, h0);
+  const int nh = segment_heads(a, seg, b, hc, h0);
   const int h = (int)blockIdx.y * kMergeWaves + (threadIdx.x >> 6);
   if (h >= nh) return;
   const size_t slot_floats = (size_t)a.heads * kPitch;
-  // Workgroups without a share between the first and the last have no piece;
-  // there are none (shares go to the first workgroups), so every one counts.
+  // (Shares go to the first workgroups, so all from `from` to wg have a piece.)
   const auto state = [&](int w) {
     return a.states + ((size_t)w * 2 + (w == from ? 1 : 0)) * slot_floats + h * kPitch;
   };
-  float mloc = kNegInf;
+  // 32 pieces at a time: their rows and, a piece to a lane, their m and l go out
+  // together with the loads of all maxima, so that up to 32 pieces take one
+  // round trip.
+  constexpr int kBatch = 32;
+  float mloc = kNegInf, M = kNegInf;
   for (int w = from + lane; w <= wg; w += 64) mloc = fmaxf(mloc, state(w)[kDim]);
-  const float M = wave_max(mloc);
   float L = 0.f, x = 0.f, y = 0.f;
-  constexpr int kBatch = 8;
   for (int w0 = from; w0 <= wg; w0 += kBatch) {
-    float2 v[kBatch], ml[kBatch];
+    float2 v[kBatch];
+#pragma unroll
+    for (int i = 0; i < kBatch; ++i)
+      v[i] = reinterpret_cast<const float2*>(state(min(w0 + i, wg)))[lane];
+    const float2 ml =
+        *reinterpret_cast<const float2*>(state(min(w0 + (lane & (kBatch - 1)), wg)) + kDim);
+    if (w0 == from) M = wave_max(mloc);
+    const float fl = M == kNegInf ? 0.f : exp2_fast(ml.x - M);
 #pragma unroll
     for (int i = 0; i < kBatch; ++i) {
-      const float* p = state(min(w0 + i, wg));
-      v[i] = reinterpret_cast<const float2*>(p)[lane];
-      ml[i] = *reinterpret_cast<const float2*>(p + kDim);
-    }
-#pragma unroll
-    for (int i = 0; i < kBatch; ++i) {
-      if (w0 + i > wg) break;
-      const float f = M == kNegInf ? 0.f : exp2_fast(ml[i].x - M);
-      L = fmaf(ml[i].y, f, L);
-      x = fmaf(v[i].x, f, x);
-      y = fmaf(v[i].y, f, y);
+      const float f = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(fl), i));
+      const float l = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(ml.y), i));
+      if (w0 + i <= wg) {
+        L = fmaf(l, f, L);
+        x = fmaf(v[i].x, f, x);
+        y = fmaf(v[i].y, f, y);
+      }
     }
   }
   reinterpret_cast<uint32_t*>(a.out + ((size_t)b * a.Hq + h0 + h) * kDim)[lane] =
@@ -658,11 +705,12 @@ bool shape_of(int B, int Hq, int Hkv, int num_blocks, int block_size, int max_bl
   if (num_blocks < 0 || block_size < 1 || block_size % kTileTokens != 0 || max_blocks < 1)
     return false;
   const int64_t cap = num_blocks == 0 ? 0 : (int64_t)block_size * max_blocks;
-  // Token positions and the batch's units fit 31 bits.
-  if (cap > INT32_MAX - kUnit || (int64_t)B * ((cap + kUnit - 1) / kUnit) > INT32_MAX) return false;
-  if ((int64_t)B * Hq > (int64_t(1) << 28)) return false;
   s.G = Hq / Hkv;
   s.chunks = (s.G + 15) / 16;
+  // Token positions and the batch's units fit 31 bits.
+  if (cap > INT32_MAX - kUnit || B * ((cap + kUnit - 1) / kUnit) > INT32_MAX / (Hkv * s.chunks))
+    return false;
+  if ((int64_t)B * Hq > (int64_t(1) << 28)) return false;
   s.heads = std::min(s.G, 16);
   s.capacity = (int)cap;
   s.per_segment = num_workgroups <= 0 && (cap + kUnit - 1) / kUnit <= kAloneUnits;
@@ -729,6 +777,7 @@ extern "C" int kv_decode_mxfp4_launch(const uint16_t* q, const uint8_t* mxfp4_ca
   a.max_blocks = max_blocks;
   a.capacity = s.capacity;
   a.tile_div = make_fastdiv((uint32_t)a.tiles_per_block);
+  a.head_div = make_fastdiv((uint32_t)(Hkv * s.chunks));
   // (A scale of 0 weighs all tokens alike; the smallest normal does as well and
   // keeps 0 * infinity out of the kernel.)
   a.scale = std::max(fabsf(scale) * gqa::kLog2e, 1.17549435e-38f);
