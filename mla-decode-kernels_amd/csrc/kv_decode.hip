@@ -102,23 +102,36 @@ struct Query {
   int scale[kWide ? 2 : 1];
 };
 
-// The queries of heads h0 .. h0 + nh - 1 of request b as the B operand: lane
-// (c, g), bytes 0-15: dims 16g .., bytes 16-31: dims 64 + 16g ...
+// The queries of heads h0 .. h0 + nh - 1 of request b, a head to each column:
+// lane (c, g), first 32 bytes: dims 16g .., then: dims 64 + 16g ...
+struct RawQuery {
+  uint4 w[4];
+};
 template <bool kWide>
-__device__ __forceinline__ Query<kWide> load_query(const DecodeArgs& a, int b, int h0, int nh,
-                                                   int c, int g) {
+__device__ __forceinline__ RawQuery load_query(const DecodeArgs& a, int b, int h0, int nh, int c,
+                                               int g) {
   const int head = kWide ? c : (c & 7);
+  RawQuery r;
+#pragma unroll
+  for (int part = 0; part < 4; ++part) {
+    r.w[part] = make_uint4(0, 0, 0, 0);
+    if (head < nh)
+      r.w[part] = *reinterpret_cast<const uint4*>(
+          a.q + ((size_t)b * a.Hq + h0 + head) * kDim + (part >> 1) * 64 + 16 * g + 8 * (part & 1));
+  }
+  return r;
+}
+
+// The same as the B operand, in two e4m3 parts.
+template <bool kWide>
+__device__ __forceinline__ Query<kWide> split_query(const RawQuery& r, float sign, int c) {
   float x[32];
 #pragma unroll
   for (int part = 0; part < 4; ++part) {
-    uint4 w = make_uint4(0, 0, 0, 0);
-    if (head < nh)
-      w = *reinterpret_cast<const uint4*>(a.q + ((size_t)b * a.Hq + h0 + head) * kDim +
-                                          (part >> 1) * 64 + 16 * g + 8 * (part & 1));
     float y[8];
-    unpack8(w, y);
+    unpack8(r.w[part], y);
 #pragma unroll
-    for (int e = 0; e < 8; ++e) x[8 * part + e] = y[e] * a.sign;
+    for (int e = 0; e < 8; ++e) x[8 * part + e] = y[e] * sign;
   }
   float top = 0.f;
 #pragma unroll
@@ -319,59 +332,51 @@ __device__ __forceinline__ void fold_unit(const Unit& u, const int (&valid)[2],
   two_dims(std::integral_constant<int, 3>{});
 }
 
-// Units [u0, u1) of a segment. The next unit's loads go out before a unit is
-// folded.
-template <bool kWide>
-__device__ __forceinline__ void scan_piece(const DecodeArgs& a, const_ints table, int head, int len,
-                                           int u0, int u1, const Query<kWide>& q, int lane,
-                                           State<kWide>& st) {
-  const int c = lane & 15, g = lane >> 4;
-  st.m = kNegInf;
-  st.l = f32x4_t{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-  for (int j = 0; j < 8; ++j) st.o[j] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-  const auto fold = [&](const Unit& u, const Spot& s) {
-    if (s.valid[0] + s.valid[1] == kUnit)
-      fold_unit<kWide, false>(u, s.valid, q, a.scale, c, g, st);
-    else
-      fold_unit<kWide, true>(u, s.valid, q, a.scale, c, g, st);
-  };
-  Unit x0, x1;
-  Spot s0 = find_unit(a, table, head, len, u0), s1;
-  load_unit(s0, lane, x0);
-  s1 = find_unit(a, table, head, len, min(u0 + 1, u1 - 1));
-  int u = u0;
-  while (true) {
-    // Past the end the last unit is loaded once more, and not folded.
-    load_unit(s1, lane, x1);
-    const Spot s2 = find_unit(a, table, head, len, min(u + 2, u1 - 1));
-    fold(x0, s0);
-    if (++u >= u1) break;
-    load_unit(s2, lane, x0);
-    s0 = s2;
-    const Spot s3 = find_unit(a, table, head, len, min(u + 2, u1 - 1));
-    fold(x1, s1);
-    s1 = s3;
-    if (++u >= u1) break;
-  }
-}
-
 // out = acc / l; a segment without a single token gets zeros.
 __device__ __forceinline__ float normal(float acc, float l) { return l == 0.f ? 0.f : acc / l; }
 
-__device__ __forceinline__ int segment_heads(const DecodeArgs& a, int seg, int& b, int& hc, int& h0) {
-  const int Hc = a.Hkv * a.chunks;
-  b = (int)fastdiv((uint32_t)seg, a.head_div);
-  hc = seg - b * Hc;
+// The q-heads of segment (b, hc): h0 .. h0 + the result - 1.
+__device__ __forceinline__ int heads_of(const DecodeArgs& a, int hc, int& h0) {
   const int kv_head = hc / a.chunks, first = (hc - kv_head * a.chunks) * 16;
   h0 = kv_head * a.G + first;
   return min(16, a.G - first);
+}
+__device__ __forceinline__ int segment_heads(const DecodeArgs& a, int seg, int& b, int& h0) {
+  b = (int)fastdiv((uint32_t)seg, a.head_div);
+  return heads_of(a, seg - b * a.Hkv * a.chunks, h0);
 }
 
 __device__ __forceinline__ int length_of(const DecodeArgs& a, int b) {
   return min(max(((const_ints)a.seq_lens)[b], 0), a.capacity);
 }
 __device__ __forceinline__ int units_of(int len) { return (int)(((uint32_t)len + kUnit - 1) / kUnit); }
+
+// A place in the line of units: unit u of segment (b, hc), whose request has
+// `len` tokens, and the units left from there on.
+struct Walk {
+  int b, hc, u, len, units;
+  uint32_t left;
+};
+
+// The next segment (there is one).
+__device__ __forceinline__ void next_segment(const DecodeArgs& a, Walk& w) {
+  w.u = 0;
+  if (++w.hc < a.Hkv * a.chunks) return;
+  w.hc = 0;
+  do w.len = length_of(a, ++w.b);
+  while (w.len == 0);
+  w.units = units_of(w.len);
+}
+
+// Where the walk's unit lies; then on to the next one. At the end of the run the
+// last place is given again (its loads are not used).
+__device__ __forceinline__ Spot next_unit(const DecodeArgs& a, Walk& w, const Spot& last) {
+  if (w.left == 0) return last;
+  const Spot s = find_unit(a, (const_ints)(a.block_table + (size_t)w.b * a.max_blocks),
+                           w.hc / a.chunks, w.len, w.u);
+  if (--w.left > 0 && ++w.u == w.units) next_segment(a, w);
+  return s;
+}
 
 // Sums over the lanes up to this one (of values whose total fits 32 bits): within
 // each row of 16 by DPP shifts, then the rows' totals.
@@ -486,15 +491,53 @@ __global__ __launch_bounds__(kThreads, 2) void kv_decode_kernel(DecodeArgs a) {
 
   int flags = 0, seg_a = 0, seg_z = 0;
   const size_t slot_floats = (size_t)a.heads * kPitch;
-  while (n > 0) {
-    const int units = units_of(len);
-    const int u1 = (int)min((uint32_t)units, u + n);
-    const int kv_head = hc / a.chunks, first = (hc - kv_head * a.chunks) * 16;
-    const int h0 = kv_head * a.G + first, nh = min(16, a.G - first);
-    const Query<kWide> q = load_query<kWide>(a, b, h0, nh, c, g);
+  if (n > 0) {
+  // Two walks over the run: `ahead` loads, `at` folds. x0 holds the next unit to
+  // fold, s1 the place of the one after it; neither stops at a segment's end.
+  Walk at{b, hc, u, len, units_of(len), n}, ahead = at;
+  Unit x0, x1;
+  Spot s0 = next_unit(a, ahead, Spot{}), s1;
+  load_unit(s0, lane, x0);
+  s1 = next_unit(a, ahead, s0);
+  int h0, nh = heads_of(a, at.hc, h0);
+  RawQuery raw = load_query<kWide>(a, at.b, h0, nh, c, g);
+  while (true) {
+    const int u0 = at.u, u1 = (int)min((uint32_t)at.units, u0 + at.left);
+    const int seg = at.b * Hc + at.hc, units = at.units;
+    uint16_t* const out = a.out + ((size_t)at.b * a.Hq + h0) * kDim;
+    const int heads = nh;
+    const Query<kWide> q = split_query<kWide>(raw, a.sign, c);
+    at.left -= (uint32_t)(u1 - u0);
+    if (at.left > 0) {  // the next segment's queries are on their way meanwhile
+      next_segment(a, at);
+      nh = heads_of(a, at.hc, h0);
+      raw = load_query<kWide>(a, at.b, h0, nh, c, g);
+    }
     State<kWide> st;
-    scan_piece<kWide>(a, (const_ints)(a.block_table + (size_t)b * a.max_blocks), kv_head, len, u,
-                      u1, q, lane, st);
+    st.m = kNegInf;
+    st.l = f32x4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int j = 0; j < 8; ++j) st.o[j] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+    const auto fold = [&](const Unit& x, const Spot& s) {
+      if (s.valid[0] + s.valid[1] == kUnit)
+        fold_unit<kWide, false>(x, s.valid, q, a.scale, c, g, st);
+      else
+        fold_unit<kWide, true>(x, s.valid, q, a.scale, c, g, st);
+    };
+    for (int k = u1 - u0;;) {
+      load_unit(s1, lane, x1);
+      const Spot s2 = next_unit(a, ahead, s1);
+      fold(x0, s0);
+      if (--k == 0) {
+        x0 = x1, s0 = s1, s1 = s2;
+        break;
+      }
+      load_unit(s2, lane, x0);
+      const Spot s3 = next_unit(a, ahead, s2);
+      fold(x1, s1);
+      s0 = s2, s1 = s3;
+      if (--k == 0) break;
+    }
     if constexpr (!kWide) {
       st.l += f32x4_t{dpp_f32<0x128>(st.l[0]), 0.f, 0.f, 0.f};
 #pragma unroll
@@ -503,9 +546,9 @@ __global__ __launch_bounds__(kThreads, 2) void kv_decode_kernel(DecodeArgs a) {
         for (int e = 0; e < 4; ++e) st.o[j][e] += dpp_f32<0x128>(st.o[j][e]);
     }
     const float l = st.l[0];
-    if (u == 0 && u1 == units) {
-      if (c < nh) {
-        uint16_t* dst = a.out + ((size_t)b * a.Hq + h0 + c) * kDim + 32 * g;
+    if (u0 == 0 && u1 == units) {
+      if (c < heads) {
+        uint16_t* dst = out + c * kDim + 32 * g;
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           float y[8];
@@ -515,15 +558,15 @@ __global__ __launch_bounds__(kThreads, 2) void kv_decode_kernel(DecodeArgs a) {
         }
       }
     } else {
-      const int which = u > 0 ? 0 : 1;
+      const int which = u0 > 0 ? 0 : 1;
       if (which == 0) {
         flags |= kHasA | (u1 == units ? kEndsA : 0);
-        seg_a = b * Hc + hc;
+        seg_a = seg;
       } else {
         flags |= kHasZ;
-        seg_z = b * Hc + hc;
+        seg_z = seg;
       }
-      if (c < nh) {
+      if (c < heads) {
         float* dst = slots + (wave * 2 + which) * slot_floats + c * kPitch;
 #pragma unroll
         for (int e = 0; e < 4; ++e)
@@ -537,14 +580,8 @@ __global__ __launch_bounds__(kThreads, 2) void kv_decode_kernel(DecodeArgs a) {
         }
       }
     }
-    n -= (uint32_t)(u1 - u);
-    if (n == 0) break;
-    u = 0;
-    if (++hc == Hc) {
-      hc = 0;
-      do len = length_of(a, ++b);
-      while (len == 0);
-    }
+    if (at.left == 0) break;
+  }
   }
   if (lane == 0) meta[wave] = Record{flags, seg_a, seg_z, 0};
   __syncthreads();
@@ -577,8 +614,8 @@ __global__ __launch_bounds__(kThreads, 2) void kv_decode_kernel(DecodeArgs a) {
       rec.flags |= kHasZ;
       rec.seg_z = seg;
     }
-    int sb, shc, h0;
-    const int nh = segment_heads(a, seg, sb, shc, h0);
+    int sb, h0;
+    const int nh = segment_heads(a, seg, sb, h0);
     int h = (wave - turn) & (kWaves - 1);
     turn += nh;
     for (; h < nh; h += kWaves) {
@@ -651,8 +688,8 @@ __global__ __launch_bounds__(64 * kMergeWaves) void kv_decode_merge_kernel(Decod
     base -= 64;
     if (base < 0) return;
   }
-  int b, hc, h0;
-  const int nh = segment_heads(a, seg, b, hc, h0);
+  int b, h0;
+  const int nh = segment_heads(a, seg, b, h0);
   const int h = (int)blockIdx.y * kMergeWaves + (threadIdx.x >> 6);
   if (h >= nh) return;
   const size_t slot_floats = (size_t)a.heads * kPitch;
@@ -713,10 +750,12 @@ bool shape_of(int B, int Hq, int Hkv, int num_blocks, int block_size, int max_bl
   if ((int64_t)B * Hq > (int64_t(1) << 28)) return false;
   s.heads = std::min(s.G, 16);
   s.capacity = (int)cap;
-  s.per_segment = num_workgroups <= 0 && (cap + kUnit - 1) / kUnit <= kAloneUnits;
+  const int64_t segments = (int64_t)B * Hkv * s.chunks;
+  s.per_segment = num_workgroups <= 0 && (cap + kUnit - 1) / kUnit <= kAloneUnits &&
+                  segments <= gqa::device_cu_count();
   s.workgroups = num_workgroups;
   if (s.per_segment)
-    s.workgroups = B * Hkv * s.chunks;
+    s.workgroups = (int)segments;
   else if (num_workgroups <= 0)
     s.workgroups = gqa::device_cu_count();
   return s.workgroups <= (1 << 22);
