@@ -58,6 +58,10 @@ constexpr int kUnit = 32;       // tokens a wave takes at a time
 constexpr int kWaves = 8;       // waves of a workgroup
 constexpr int kThreads = 64 * kWaves;
 constexpr int kPitch = 132;     // floats of a head's state: acc [128], m, l, pad
+#ifndef KV_AHEAD
+#define KV_AHEAD 1
+#endif
+constexpr int kAhead = KV_AHEAD;       // units whose loads are in flight while one is folded
 constexpr int kMinUnits = 2;    // units a wave gets before another workgroup joins in
 
 constexpr int kHasA = 1, kEndsA = 2, kHasZ = 4;  // pieces of a share (Record::flags)
@@ -87,6 +91,7 @@ struct DecodeArgs {
 struct Unit {
   uint4 k[2], v[2];
   uint32_t ks[2], vs[2];
+  int valid[2];  // tokens of each tile that count (0 .. 16)
 };
 
 template <bool kWide>
@@ -173,34 +178,31 @@ __device__ __forceinline__ Query<kWide> split_query(const RawQuery& r, float sig
   return q;
 }
 
-// Where a unit's two tiles lie, and which of its tokens count.
-struct Spot {
-  const uint8_t* tile[2];
-  int valid[2];  // tokens of each tile that count (0 .. 16)
-};
-
 // Block ids through the constant address space: scalar loads, which do not
 // share a counter with the tiles' loads (as gqa_scan_mfma.hpp measured).
 typedef const __attribute__((address_space(4))) int* const_ints;
+
+// Where a unit's two tiles are to be found, the block ids on their way: nothing
+// looks at them before the unit's loads go out, a unit later, so their latency
+// hides behind a fold.
+struct Spot {
+  int id[2];
+  uint32_t tile[2];  // the tile's number in a block of all heads' tiles
+  int valid[2];      // tokens of each tile that are below the length (0 .. 16)
+};
 
 __device__ __forceinline__ Spot find_unit(const DecodeArgs& a, const_ints table, int head, int len,
                                           int u) {
   Spot s;
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
+    // (A second tile past the end: the first one once more, no token of it.)
     const int first = u * kUnit + h * kTileTokens;
     s.valid[h] = min(max(len - first, 0), kTileTokens);
-    s.tile[h] = h ? s.tile[0] : a.cache;
-    if (s.valid[h] == 0) continue;  // past the end: any tile that may be read
-    const uint32_t t = (uint32_t)first / kTileTokens;
+    const uint32_t t = 2 * (uint32_t)u + (s.valid[h] > 0 ? h : 0);
     const uint32_t lb = fastdiv(t, a.tile_div);
-    const int id = table[lb];
-    if ((uint32_t)id >= (uint32_t)a.num_blocks) {
-      s.valid[h] = 0;
-      continue;
-    }
-    s.tile[h] = a.cache + (((size_t)id * a.Hkv + head) * a.tiles_per_block +
-                           (t - lb * a.tile_div.d)) * kTileBytes;
+    s.id[h] = table[lb];
+    s.tile[h] = (uint32_t)head * a.tiles_per_block + (t - lb * a.tile_div.d);
   }
   return s;
 }
@@ -210,10 +212,16 @@ __device__ __forceinline__ uint4 stream16(const uint8_t* p) {
   return make_uint4(v.x, v.y, v.z, v.w);
 }
 
-__device__ __forceinline__ void load_unit(const Spot& s, int lane, Unit& u) {
+__device__ __forceinline__ void load_unit(const DecodeArgs& a, const Spot& s, uint32_t lane,
+                                          Unit& u) {
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
-    const uint8_t* p = s.tile[h];
+    // An id outside the cache: block 0 is read, no token of it counts.
+    const bool in = (uint32_t)s.id[h] < (uint32_t)a.num_blocks;
+    u.valid[h] = in ? s.valid[h] : 0;
+    const uint8_t* p =
+        a.cache + ((size_t)(in ? s.id[h] : 0) * ((uint32_t)a.Hkv * a.tiles_per_block) + s.tile[h]) *
+                      kTileBytes;
     u.k[h] = stream16(p + 16 * lane);
     u.v[h] = stream16(p + kValueCodes + 16 * lane);
     u.ks[h] = p[kKeyScales + lane];
@@ -224,9 +232,9 @@ __device__ __forceinline__ void load_unit(const Spot& s, int lane, Unit& u) {
 
 // Fold a unit into the state. kMask: some of its tokens do not count.
 template <bool kWide, bool kMask>
-__device__ __forceinline__ void fold_unit(const Unit& u, const int (&valid)[2],
-                                          const Query<kWide>& q, float scale, int c, int g,
-                                          State<kWide>& st) {
+__device__ __forceinline__ void fold_unit(const Unit& u, const Query<kWide>& q, float scale, int c,
+                                          int g, State<kWide>& st) {
+  const int (&valid)[2] = u.valid;
   float s[8];
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
@@ -369,13 +377,12 @@ __device__ __forceinline__ void next_segment(const DecodeArgs& a, Walk& w) {
 }
 
 // Where the walk's unit lies; then on to the next one. At the end of the run the
-// last place is given again (its loads are not used).
-__device__ __forceinline__ Spot next_unit(const DecodeArgs& a, Walk& w, const Spot& last) {
-  if (w.left == 0) return last;
-  const Spot s = find_unit(a, (const_ints)(a.block_table + (size_t)w.b * a.max_blocks),
+// last place stays (its loads are not used).
+__device__ __forceinline__ void next_unit(const DecodeArgs& a, Walk& w, Spot& s) {
+  if (w.left == 0) return;
+  s = find_unit(a, (const_ints)(a.block_table + (size_t)w.b * a.max_blocks),
                            w.hc / a.chunks, w.len, w.u);
   if (--w.left > 0 && ++w.u == w.units) next_segment(a, w);
-  return s;
 }
 
 // Sums over the lanes up to this one (of values whose total fits 32 bits): within
@@ -407,13 +414,6 @@ __global__ __launch_bounds__(kThreads, 2) void kv_decode_kernel(DecodeArgs a) {
   const int c = lane & 15, g = lane >> 4;
   const int Hc = a.Hkv * a.chunks;
   const int wg = blockIdx.x, nwg = gridDim.x;
-
-  // Requests without tokens get zeros.
-  for (int b = a.per_segment ? (int)fastdiv((uint32_t)wg, a.head_div) : wg; b < a.B; b += a.per_segment ? a.B : nwg) {
-    if (length_of(a, b) > 0) continue;
-    for (int i = tid; i < a.Hq * kDim / 8; i += kThreads)
-      reinterpret_cast<uint4*>(a.out + (size_t)b * a.Hq * kDim)[i] = make_uint4(0, 0, 0, 0);
-  }
 
   // This wave's run of units: it starts at unit u of segment (b, hc) and holds n.
   int b, hc, u, len;
@@ -492,13 +492,18 @@ __global__ __launch_bounds__(kThreads, 2) void kv_decode_kernel(DecodeArgs a) {
   int flags = 0, seg_a = 0, seg_z = 0;
   const size_t slot_floats = (size_t)a.heads * kPitch;
   if (n > 0) {
-  // Two walks over the run: `ahead` loads, `at` folds. x0 holds the next unit to
-  // fold, s1 the place of the one after it; neither stops at a segment's end.
+  // Two walks over the run: `ahead` loads, `at` folds. x[0 .. kAhead - 1] hold the
+  // next units to fold, `next` is the place of the one after them; neither walk
+  // stops at a segment's end.
   Walk at{b, hc, u, len, units_of(len), n}, ahead = at;
-  Unit x0, x1;
-  Spot s0 = next_unit(a, ahead, Spot{}), s1;
-  load_unit(s0, lane, x0);
-  s1 = next_unit(a, ahead, s0);
+  Unit x[kAhead + 1];
+  Spot next{};
+#pragma unroll
+  for (int i = 0; i < kAhead; ++i) {
+    next_unit(a, ahead, next);
+    load_unit(a, next, lane, x[i]);
+  }
+  next_unit(a, ahead, next);
   int h0, nh = heads_of(a, at.hc, h0);
   RawQuery raw = load_query<kWide>(a, at.b, h0, nh, c, g);
   while (true) {
@@ -518,25 +523,32 @@ __global__ __launch_bounds__(kThreads, 2) void kv_decode_kernel(DecodeArgs a) {
     st.l = f32x4_t{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int j = 0; j < 8; ++j) st.o[j] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-    const auto fold = [&](const Unit& x, const Spot& s) {
-      if (s.valid[0] + s.valid[1] == kUnit)
-        fold_unit<kWide, false>(x, s.valid, q, a.scale, c, g, st);
+    int k = u1 - u0;
+    // Unit i of the ring: the loads of the unit kAhead behind it go out, then it is
+    // folded. At the piece's end the ring is turned so that x[0] comes next.
+    const auto step = [&](auto index) {
+      constexpr int i = decltype(index)::value, kRing = kAhead + 1;
+      load_unit(a, next, lane, x[(i + kAhead) % kRing]);
+      next_unit(a, ahead, next);
+      if (x[i].valid[0] + x[i].valid[1] == kUnit)
+        fold_unit<kWide, false>(x[i], q, a.scale, c, g, st);
       else
-        fold_unit<kWide, true>(x, s.valid, q, a.scale, c, g, st);
+        fold_unit<kWide, true>(x[i], q, a.scale, c, g, st);
+      if (--k > 0) return false;
+      Unit y[kAhead];
+#pragma unroll
+      for (int j = 0; j < kAhead; ++j) y[j] = x[(i + 1 + j) % kRing];
+#pragma unroll
+      for (int j = 0; j < kAhead; ++j) x[j] = y[j];
+      return true;
     };
-    for (int k = u1 - u0;;) {
-      load_unit(s1, lane, x1);
-      const Spot s2 = next_unit(a, ahead, s1);
-      fold(x0, s0);
-      if (--k == 0) {
-        x0 = x1, s0 = s1, s1 = s2;
-        break;
-      }
-      load_unit(s2, lane, x0);
-      const Spot s3 = next_unit(a, ahead, s2);
-      fold(x1, s1);
-      s0 = s2, s1 = s3;
-      if (--k == 0) break;
+    while (true) {
+      if (step(std::integral_constant<int, 0>{})) break;
+      if (step(std::integral_constant<int, 1>{})) break;
+      if constexpr (kAhead > 1)
+        if (step(std::integral_constant<int, 2>{})) break;
+      if constexpr (kAhead > 2)
+        if (step(std::integral_constant<int, 3>{})) break;
     }
     if constexpr (!kWide) {
       st.l += f32x4_t{dpp_f32<0x128>(st.l[0]), 0.f, 0.f, 0.f};
@@ -664,6 +676,13 @@ __global__ __launch_bounds__(kThreads, 2) void kv_decode_kernel(DecodeArgs a) {
     for (uint32_t left = has_z; left; left &= left - 1) fold_run(__builtin_ctz(left), 1);
   }
   if (!a.per_segment && tid == 0) a.records[wg] = rec;
+
+  // Requests without tokens get zeros.
+  for (int b = a.per_segment ? (int)fastdiv((uint32_t)wg, a.head_div) : wg; b < a.B; b += a.per_segment ? a.B : nwg) {
+    if (length_of(a, b) > 0) continue;
+    for (int i = tid; i < a.Hq * kDim / 8; i += kThreads)
+      reinterpret_cast<uint4*>(a.out + (size_t)b * a.Hq * kDim)[i] = make_uint4(0, 0, 0, 0);
+  }
 }
 
 // Segments cut between workgroups: the workgroup whose first piece ends one
