@@ -230,27 +230,51 @@ __device__ __forceinline__ void load_unit(const DecodeArgs& a, const Spot& s, ui
   }
 }
 
-// Fold a unit into the state. kMask: some of its tokens do not count.
-template <bool kWide, bool kMask>
-__device__ __forceinline__ void fold_unit(const Unit& u, const Query<kWide>& q, float scale, int c,
-                                          int g, State<kWide>& st) {
-  const int (&valid)[2] = u.valid;
+// What takes tokens out of a unit, in registers that stay the same while units
+// are whole: the C operand of QK^T (-infinity for a token that does not count),
+// and bytes that hide the scales of those tokens, which may be anything (255
+// would make them NaN), behind a scale of 1.
+struct Mask {
+  f32x4_t bias[2];
+  uint32_t ks[2], vs[2];
+};
+
+__device__ __forceinline__ void set_mask(Mask& m, const int (&valid)[2], int c, int g) {
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    m.ks[h] = c < valid[h] ? 0xffu : 0u;
+    m.vs[h] = 0;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const bool in = 4 * g + e < valid[h];
+      m.bias[h][e] = in ? 0.f : kNegInf;
+      m.vs[h] |= in ? 0xffu << (8 * e) : 0u;
+    }
+  }
+}
+
+__device__ __forceinline__ uint32_t select_bits(uint32_t mask, uint32_t x, uint32_t y) {
+  return (x & mask) | (y & ~mask);
+}
+
+// Fold a unit into the state.
+template <bool kWide>
+__device__ __forceinline__ void fold_unit(const Unit& u, const Mask& mask, const Query<kWide>& q,
+                                          float scale, int c, State<kWide>& st) {
   float s[8];
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
     const i32x8_t k = {(int)u.k[h].x, (int)u.k[h].y, (int)u.k[h].z, (int)u.k[h].w, 0, 0, 0, 0};
-    f32x4_t d = {0.f, 0.f, 0.f, 0.f};
-    d = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(k, q.part[0], d, 4, 0, 0, (int)u.ks[h], 0,
-                                                         q.scale[0]);
+    const int ks = (int)select_bits(mask.ks[h], u.ks[h], 127u);
+    f32x4_t d = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(k, q.part[0], mask.bias[h], 4, 0, 0,
+                                                                 ks, 0, q.scale[0]);
     if constexpr (kWide)
-      d = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(k, q.part[1], d, 4, 0, 0,
-                                                           (int)u.ks[h], 0, q.scale[1]);
+      d = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(k, q.part[1], d, 4, 0, 0, ks, 0,
+                                                           q.scale[1]);
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
+    for (int e = 0; e < 4; ++e)
       // Columns c and c + 8 hold the two parts: a rotation by 8 within the row.
       s[4 * h + e] = kWide ? d[e] : d[e] + dpp_f32<0x128>(d[e]);
-      if (kMask && 4 * g + e >= valid[h]) s[4 * h + e] = kNegInf;
-    }
   }
   float mx = s[0];
 #pragma unroll
@@ -264,13 +288,12 @@ __device__ __forceinline__ void fold_unit(const Unit& u, const Query<kWide>& q, 
 #pragma unroll
     for (int j = 0; j < 8; ++j) st.o[j] *= alpha;
   }
-  const float ms = kMask && st.m == kNegInf ? 0.f : st.m * scale;
+  const float ms = st.m == kNegInf ? 0.f : st.m * scale;
   uint32_t p[kWide ? 2 : 1][8];
   const uint32_t low = kWide || c < 8 ? 0u : 0xffff0000u;
 #pragma unroll
   for (int e = 0; e < 8; ++e) {
-    float w = exp2_fast(fmaf(s[e], scale, -ms));
-    if (kMask && s[e] == kNegInf) w = 0.f;
+    const float w = exp2_fast(fmaf(s[e], scale, -ms));
     const uint32_t bits = __float_as_uint(w);
     if constexpr (kWide) {
       p[0][e] = bits;
@@ -293,15 +316,11 @@ __device__ __forceinline__ void fold_unit(const Unit& u, const Query<kWide>& q, 
   float vs[8];
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
-    vs[4 * h + 0] = __uint_as_float(u.vs[h] << 23);
-    vs[4 * h + 1] = __uint_as_float(u.vs[h] << 15);
-    vs[4 * h + 2] = __uint_as_float(u.vs[h] << 7);
-    vs[4 * h + 3] = __uint_as_float(u.vs[h] >> 1);
-    if constexpr (kMask) {  // what lies behind the last token may be anything
-#pragma unroll
-      for (int e = 0; e < 4; ++e)
-        if (4 * g + e >= valid[h]) vs[4 * h + e] = 1.f;
-    }
+    const uint32_t w = select_bits(mask.vs[h], u.vs[h], 0x7f7f7f7fu);
+    vs[4 * h + 0] = __uint_as_float(w << 23);
+    vs[4 * h + 1] = __uint_as_float(w << 15);
+    vs[4 * h + 2] = __uint_as_float(w << 7);
+    vs[4 * h + 3] = __uint_as_float(w >> 1);
   }
   const uint32_t code[8] = {u.v[0].x, u.v[0].y, u.v[0].z, u.v[0].w,
                             u.v[1].x, u.v[1].y, u.v[1].z, u.v[1].w};
@@ -506,6 +525,8 @@ __global__ __launch_bounds__(kThreads, 2) void kv_decode_kernel(DecodeArgs a) {
   next_unit(a, ahead, next);
   int h0, nh = heads_of(a, at.hc, h0);
   RawQuery raw = load_query<kWide>(a, at.b, h0, nh, c, g);
+  Mask mask;
+  bool unmasked = false;
   while (true) {
     const int u0 = at.u, u1 = (int)min((uint32_t)at.units, u0 + at.left);
     const int seg = at.b * Hc + at.hc, units = at.units;
@@ -530,10 +551,12 @@ __global__ __launch_bounds__(kThreads, 2) void kv_decode_kernel(DecodeArgs a) {
       constexpr int i = decltype(index)::value, kRing = kAhead + 1;
       load_unit(a, next, lane, x[(i + kAhead) % kRing]);
       next_unit(a, ahead, next);
-      if (x[i].valid[0] + x[i].valid[1] == kUnit)
-        fold_unit<kWide, false>(x[i], q, a.scale, c, g, st);
-      else
-        fold_unit<kWide, true>(x[i], q, a.scale, c, g, st);
+      const bool whole = x[i].valid[0] + x[i].valid[1] == kUnit;
+      if (!whole || !unmasked) {
+        set_mask(mask, x[i].valid, c, g);
+        unmasked = whole;
+      }
+      fold_unit<kWide>(x[i], mask, q, a.scale, c, st);
       if (--k > 0) return false;
       Unit y[kAhead];
 #pragma unroll
