@@ -58,16 +58,19 @@ constexpr int kUnit = 32;       // tokens a wave takes at a time
 constexpr int kWaves = 8;       // waves of a workgroup
 constexpr int kThreads = 64 * kWaves;
 constexpr int kPitch = 132;     // floats of a head's state: acc [128], m, l, pad
-#ifndef KV_AHEAD
-#define KV_AHEAD 1
-#endif
-constexpr int kAhead = KV_AHEAD;       // units whose loads are in flight while one is folded
 constexpr int kMinUnits = 2;    // units a wave gets before another workgroup joins in
 
 constexpr int kHasA = 1, kEndsA = 2, kHasZ = 4;  // pieces of a share (Record::flags)
 
 struct Record {
   int flags, seg_a, seg_z, pad;
+};
+
+// How the units are shared out.
+enum : int {
+  kBalanced,    // equal runs to all workgroups, cutting segments (two launches)
+  kWhole,       // the same, each workgroup's ends moved to the next segment's start
+  kPerSegment,  // a workgroup for each segment, its units dealt out to the waves in turn
 };
 
 struct DecodeArgs {
@@ -84,7 +87,7 @@ struct DecodeArgs {
   FastDiv head_div;  // by Hkv * chunks
   float scale;       // |scale| log2(e)
   float sign;        // of scale
-  int per_segment;   // a workgroup for each segment: no shares, nothing in the workspace
+  int mode;
 };
 
 // A unit's data in registers.
@@ -379,9 +382,9 @@ __device__ __forceinline__ int length_of(const DecodeArgs& a, int b) {
 __device__ __forceinline__ int units_of(int len) { return (int)(((uint32_t)len + kUnit - 1) / kUnit); }
 
 // A place in the line of units: unit u of segment (b, hc), whose request has
-// `len` tokens, and the units left from there on.
+// `len` tokens, and the units left from there on (`step` apart in the segment).
 struct Walk {
-  int b, hc, u, len, units;
+  int b, hc, u, len, units, step;
   uint32_t left;
 };
 
@@ -395,13 +398,16 @@ __device__ __forceinline__ void next_segment(const DecodeArgs& a, Walk& w) {
   w.units = units_of(w.len);
 }
 
+__device__ __forceinline__ const_ints table_of(const DecodeArgs& a, int b) {
+  return (const_ints)(a.block_table + (size_t)b * a.max_blocks);
+}
+
 // Where the walk's unit lies; then on to the next one. At the end of the run the
 // last place stays (its loads are not used).
 __device__ __forceinline__ void next_unit(const DecodeArgs& a, Walk& w, Spot& s) {
   if (w.left == 0) return;
-  s = find_unit(a, (const_ints)(a.block_table + (size_t)w.b * a.max_blocks),
-                           w.hc / a.chunks, w.len, w.u);
-  if (--w.left > 0 && ++w.u == w.units) next_segment(a, w);
+  s = find_unit(a, table_of(a, w.b), w.hc / a.chunks, w.len, w.u);
+  if (--w.left > 0 && (w.u += w.step) >= w.units) next_segment(a, w);
 }
 
 // Sums over the lanes up to this one (of values whose total fits 32 bits): within
@@ -434,16 +440,31 @@ __global__ __launch_bounds__(kThreads, 2) void kv_decode_kernel(DecodeArgs a) {
   const int Hc = a.Hkv * a.chunks;
   const int wg = blockIdx.x, nwg = gridDim.x;
 
-  // This wave's run of units: it starts at unit u of segment (b, hc) and holds n.
-  int b, hc, u, len;
-  uint32_t n;
-  if (a.per_segment) {
-    b = (int)fastdiv((uint32_t)wg, a.head_div);
-    hc = wg - b * Hc;
-    len = length_of(a, b);
-    const uint32_t total = (uint32_t)units_of(len);
-    u = (int)(total * (uint32_t)wave / kWaves);
-    n = total * (uint32_t)(wave + 1) / kWaves - u;
+  // This wave's run of units, in two walks: `at` folds, `ahead` loads. x0 holds
+  // the next unit to fold, `next` is the place of the one after it; neither walk
+  // stops at a segment's end.
+  Walk at{};
+  Spot next{};
+  Unit x0, x1;
+  RawQuery raw;
+  if (a.mode == kPerSegment) {
+    at.b = (int)fastdiv((uint32_t)wg, a.head_div);
+    at.hc = wg - at.b * Hc;
+    at.u = wave;
+    at.step = kWaves;
+    // The first unit is loaded before its length is known (the table row is there
+    // to its end, and an id is looked at before it is used): one memory latency
+    // less in a launch that has little else.
+    if (wave < units_of(a.capacity)) {
+      next = find_unit(a, table_of(a, at.b), at.hc / a.chunks, a.capacity, wave);
+      load_unit(a, next, lane, x0);
+    }
+    at.len = length_of(a, at.b);
+    at.units = units_of(at.len);
+    at.left = wave < at.units ? (uint32_t)(at.units - wave + kWaves - 1) / kWaves : 0;
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+      x0.valid[h] = min(x0.valid[h], max(at.len - wave * kUnit - h * kTileTokens, 0));
   } else {
     // Prefix sums of the requests' units, a slice of them to each lane of one
     // wave (every wave for itself), or to each thread of the workgroup.
@@ -476,147 +497,147 @@ __global__ __launch_bounds__(kThreads, 2) void kv_decode_kernel(DecodeArgs a) {
     const uint32_t want = max(1u, (all + kWaves * kMinUnits - 1) / (kWaves * kMinUnits));
     const uint32_t used = min(want, (uint32_t)nwg);
     const uint32_t each = all / used, more = all - each * used;
-    const uint32_t w0 = (uint32_t)wg * each + min((uint32_t)wg, more);
-    const uint32_t share = (uint32_t)wg < used ? each + ((uint32_t)wg < more ? 1 : 0) : 0;
-    const uint32_t p0 = w0 + (uint32_t)((uint64_t)share * wave / kWaves);
-    n = w0 + (uint32_t)((uint64_t)share * (wave + 1) / kWaves) - p0;
-    b = hc = u = len = 0;
-    if (n > 0) {
-      // The slice that holds unit x, then the request in it.
-      const uint32_t x = fastdiv(p0, a.head_div);
+    // Unit p of the line as a place; the request is the one whose prefix sum holds
+    // unit p / Hc of a single head.
+    const auto locate = [&](uint32_t p, Walk& w) {
+      const uint32_t x = fastdiv(p, a.head_div);
       int found = 0;
       uint32_t pre;
       if (small) {
-        const uint32_t mine_before = inc - sum;
-        found = __popcll(__builtin_amdgcn_ballot_w64(mine_before <= x));
-        pre = (uint32_t)__builtin_amdgcn_readlane((int)mine_before, found - 1);
+        const uint32_t before = inc - sum;
+        found = __popcll(__builtin_amdgcn_ballot_w64(before <= x));
+        pre = (uint32_t)__builtin_amdgcn_readlane((int)before, found - 1);
       } else {
 #pragma unroll
         for (int i = 0; i < kWaves; ++i)
           found += __popcll(__builtin_amdgcn_ballot_w64(prefix[i * 64 + lane] <= x));
         pre = (uint32_t)__builtin_amdgcn_readfirstlane((int)prefix[found - 1]);
       }
-      b = __builtin_amdgcn_readfirstlane((found - 1) * slice);
-      len = length_of(a, b);
-      while (x - pre >= (uint32_t)units_of(len)) {
-        pre += (uint32_t)units_of(len);
-        len = length_of(a, ++b);
+      w.b = __builtin_amdgcn_readfirstlane((found - 1) * slice);
+      w.len = length_of(a, w.b);
+      w.units = units_of(w.len);
+      while (x - pre >= (uint32_t)w.units) {
+        pre += (uint32_t)w.units;
+        w.len = length_of(a, ++w.b);
+        w.units = units_of(w.len);
       }
-      const uint32_t rem = p0 - pre * (uint32_t)Hc, units = (uint32_t)units_of(len);
-      hc = (int)(rem / units);
-      u = (int)(rem - (uint32_t)hc * units);
+      const uint32_t rem = p - pre * (uint32_t)Hc;
+      w.hc = (int)(rem / (uint32_t)w.units);
+      w.u = (int)(rem - (uint32_t)w.hc * (uint32_t)w.units);
+    };
+    at.step = 1;
+    uint32_t w0 = (uint32_t)wg * each + min((uint32_t)wg, more);
+    uint32_t w1 = (uint32_t)wg < used ? w0 + each + ((uint32_t)wg < more ? 1 : 0) : w0;
+    if (a.mode == kWhole && w0 < w1) {
+      locate(w0, at);
+      if (at.u > 0) w0 += (uint32_t)(at.units - at.u);
+      if (w1 < all) {
+        locate(w1, at);
+        if (at.u > 0) w1 += (uint32_t)(at.units - at.u);
+      }
     }
+    const uint32_t share = w1 - w0;  // (a segment that holds a whole share: 0)
+    const uint32_t p0 = w0 + (uint32_t)((uint64_t)share * wave / kWaves);
+    at.left = w0 + (uint32_t)((uint64_t)share * (wave + 1) / kWaves) - p0;
+    if (at.left > 0) locate(p0, at);
   }
 
   int flags = 0, seg_a = 0, seg_z = 0;
   const size_t slot_floats = (size_t)a.heads * kPitch;
-  if (n > 0) {
-  // Two walks over the run: `ahead` loads, `at` folds. x[0 .. kAhead - 1] hold the
-  // next units to fold, `next` is the place of the one after them; neither walk
-  // stops at a segment's end.
-  Walk at{b, hc, u, len, units_of(len), n}, ahead = at;
-  Unit x[kAhead + 1];
-  Spot next{};
-#pragma unroll
-  for (int i = 0; i < kAhead; ++i) {
+  if (at.left > 0) {
+    Walk ahead = at;
     next_unit(a, ahead, next);
-    load_unit(a, next, lane, x[i]);
-  }
-  next_unit(a, ahead, next);
-  int h0, nh = heads_of(a, at.hc, h0);
-  RawQuery raw = load_query<kWide>(a, at.b, h0, nh, c, g);
-  Mask mask;
-  bool unmasked = false;
-  while (true) {
-    const int u0 = at.u, u1 = (int)min((uint32_t)at.units, u0 + at.left);
-    const int seg = at.b * Hc + at.hc, units = at.units;
-    uint16_t* const out = a.out + ((size_t)at.b * a.Hq + h0) * kDim;
-    const int heads = nh;
-    const Query<kWide> q = split_query<kWide>(raw, a.sign, c);
-    at.left -= (uint32_t)(u1 - u0);
-    if (at.left > 0) {  // the next segment's queries are on their way meanwhile
-      next_segment(a, at);
-      nh = heads_of(a, at.hc, h0);
-      raw = load_query<kWide>(a, at.b, h0, nh, c, g);
-    }
-    State<kWide> st;
-    st.m = kNegInf;
-    st.l = f32x4_t{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-    for (int j = 0; j < 8; ++j) st.o[j] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-    int k = u1 - u0;
-    // Unit i of the ring: the loads of the unit kAhead behind it go out, then it is
-    // folded. At the piece's end the ring is turned so that x[0] comes next.
-    const auto step = [&](auto index) {
-      constexpr int i = decltype(index)::value, kRing = kAhead + 1;
-      load_unit(a, next, lane, x[(i + kAhead) % kRing]);
-      next_unit(a, ahead, next);
-      const bool whole = x[i].valid[0] + x[i].valid[1] == kUnit;
-      if (!whole || !unmasked) {
-        set_mask(mask, x[i].valid, c, g);
-        unmasked = whole;
-      }
-      fold_unit<kWide>(x[i], mask, q, a.scale, c, st);
-      if (--k > 0) return false;
-      Unit y[kAhead];
-#pragma unroll
-      for (int j = 0; j < kAhead; ++j) y[j] = x[(i + 1 + j) % kRing];
-#pragma unroll
-      for (int j = 0; j < kAhead; ++j) x[j] = y[j];
-      return true;
-    };
+    if (a.mode != kPerSegment) load_unit(a, next, lane, x0);
+    next_unit(a, ahead, next);
+    int h0, nh = heads_of(a, at.hc, h0);
+    raw = load_query<kWide>(a, at.b, h0, nh, c, g);
+    Mask mask;
+    bool unmasked = false;
     while (true) {
-      if (step(std::integral_constant<int, 0>{})) break;
-      if (step(std::integral_constant<int, 1>{})) break;
-      if constexpr (kAhead > 1)
-        if (step(std::integral_constant<int, 2>{})) break;
-      if constexpr (kAhead > 2)
-        if (step(std::integral_constant<int, 3>{})) break;
-    }
-    if constexpr (!kWide) {
-      st.l += f32x4_t{dpp_f32<0x128>(st.l[0]), 0.f, 0.f, 0.f};
-#pragma unroll
-      for (int j = 0; j < 8; ++j)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) st.o[j][e] += dpp_f32<0x128>(st.o[j][e]);
-    }
-    const float l = st.l[0];
-    if (u0 == 0 && u1 == units) {
-      if (c < heads) {
-        uint16_t* dst = out + c * kDim + 32 * g;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          float y[8];
-#pragma unroll
-          for (int j = 0; j < 8; ++j) y[j] = normal(st.o[j][e], l);
-          *reinterpret_cast<uint4*>(dst + 8 * e) = pack8(y);
-        }
+      int k = (int)min((uint32_t)(at.units - at.u), at.left);
+      bool starts = at.u == 0, ends = at.u + k == at.units;
+      if (a.mode == kPerSegment) {
+        k = (int)at.left;
+        starts = wave == 0;
+        ends = wave == min(at.units, kWaves) - 1;
       }
-    } else {
-      const int which = u0 > 0 ? 0 : 1;
-      if (which == 0) {
-        flags |= kHasA | (u1 == units ? kEndsA : 0);
-        seg_a = seg;
+      const int seg = at.b * Hc + at.hc, heads = nh;
+      uint16_t* const out = a.out + ((size_t)at.b * a.Hq + h0) * kDim;
+      const Query<kWide> q = split_query<kWide>(raw, a.sign, c);
+      at.left -= (uint32_t)k;
+      if (at.left > 0) {  // the next segment's queries are on their way meanwhile
+        next_segment(a, at);
+        nh = heads_of(a, at.hc, h0);
+        raw = load_query<kWide>(a, at.b, h0, nh, c, g);
+      }
+      State<kWide> st;
+      st.m = kNegInf;
+      st.l = f32x4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int j = 0; j < 8; ++j) st.o[j] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+      // Unit x is folded while the loads of the one after it are in flight.
+      const auto step = [&](const Unit& x, Unit& y) {
+        load_unit(a, next, lane, y);
+        next_unit(a, ahead, next);
+        const bool whole = x.valid[0] + x.valid[1] == kUnit;
+        if (!whole || !unmasked) {
+          set_mask(mask, x.valid, c, g);
+          unmasked = whole;
+        }
+        fold_unit<kWide>(x, mask, q, a.scale, c, st);
+        return --k == 0;
+      };
+      while (true) {
+        if (step(x0, x1)) {
+          x0 = x1;
+          break;
+        }
+        if (step(x1, x0)) break;
+      }
+      if constexpr (!kWide) {
+        st.l += f32x4_t{dpp_f32<0x128>(st.l[0]), 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) st.o[j][e] += dpp_f32<0x128>(st.o[j][e]);
+      }
+      const float l = st.l[0];
+      if (starts && ends) {
+        if (c < heads) {
+          uint16_t* dst = out + c * kDim + 32 * g;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            float y[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) y[j] = normal(st.o[j][e], l);
+            *reinterpret_cast<uint4*>(dst + 8 * e) = pack8(y);
+          }
+        }
       } else {
-        flags |= kHasZ;
-        seg_z = seg;
-      }
-      if (c < heads) {
-        float* dst = slots + (wave * 2 + which) * slot_floats + c * kPitch;
+        const int which = starts ? 1 : 0;
+        if (which == 0) {
+          flags |= kHasA | (ends ? kEndsA : 0);
+          seg_a = seg;
+        } else {
+          flags |= kHasZ;
+          seg_z = seg;
+        }
+        if (c < heads) {
+          float* dst = slots + (wave * 2 + which) * slot_floats + c * kPitch;
 #pragma unroll
-        for (int e = 0; e < 4; ++e)
+          for (int e = 0; e < 4; ++e)
 #pragma unroll
-          for (int j = 0; j < 8; j += 4)
-            *reinterpret_cast<f32x4_t*>(dst + 32 * g + 8 * e + j) =
-                f32x4_t{st.o[j][e], st.o[j + 1][e], st.o[j + 2][e], st.o[j + 3][e]};
-        if (g == 0) {
-          dst[kDim] = st.m == kNegInf ? kNegInf : st.m * a.scale;
-          dst[kDim + 1] = l;
+            for (int j = 0; j < 8; j += 4)
+              *reinterpret_cast<f32x4_t*>(dst + 32 * g + 8 * e + j) =
+                  f32x4_t{st.o[j][e], st.o[j + 1][e], st.o[j + 2][e], st.o[j + 3][e]};
+          if (g == 0) {
+            dst[kDim] = st.m == kNegInf ? kNegInf : st.m * a.scale;
+            dst[kDim + 1] = l;
+          }
         }
       }
+      if (at.left == 0) break;
     }
-    if (at.left == 0) break;
-  }
   }
   if (lane == 0) meta[wave] = Record{flags, seg_a, seg_z, 0};
   __syncthreads();
@@ -633,7 +654,15 @@ __global__ __launch_bounds__(kThreads, 2) void kv_decode_kernel(DecodeArgs a) {
   const uint32_t has_a = bits(kHasA), ends_a = bits(kEndsA), has_z = bits(kHasZ);
   Record rec{0, 0, 0, 0};
   int turn = 0;  // heads handed out so far
-  const auto fold_run = [&](int w, int which) {
+  // (A first wave with a cut piece that has no A piece starts at a segment's
+  // start, as those in front of it then did, empty or not.)
+  const uint32_t any = has_a | has_z;
+  uint32_t runs = has_z;  // the waves whose Z starts a run ..
+  int which = 1, w = 0;
+  if (any && (has_a >> __builtin_ctz(any) & 1)) which = 0;  // .. and the A in front
+  while (which == 0 || runs) {
+    w = __builtin_ctz(which ? runs : any);
+    if (which) runs &= runs - 1;
     // From wave w's piece on: A pieces up to the first that ends its segment.
     const uint32_t behind = which ? ~((2u << w) - 1) : ~((1u << w) - 1);
     const uint32_t last = ends_a & behind;
@@ -689,19 +718,14 @@ __global__ __launch_bounds__(kThreads, 2) void kv_decode_kernel(DecodeArgs a) {
         if (lane == 0) reinterpret_cast<float2*>(dst + kDim)[0] = make_float2(M, L);
       }
     }
-  };
-  // (A first wave with a cut piece that has no A piece starts at a segment's
-  // start, as those in front of it then did, empty or not.)
-  const uint32_t any = has_a | has_z;
-  if (any) {
-    const int first = __builtin_ctz(any);
-    if (has_a >> first & 1) fold_run(first, 0);
-    for (uint32_t left = has_z; left; left &= left - 1) fold_run(__builtin_ctz(left), 1);
+    which = 1;
   }
-  if (!a.per_segment && tid == 0) a.records[wg] = rec;
+  if (a.mode == kBalanced && tid == 0) a.records[wg] = rec;
 
   // Requests without tokens get zeros.
-  for (int b = a.per_segment ? (int)fastdiv((uint32_t)wg, a.head_div) : wg; b < a.B; b += a.per_segment ? a.B : nwg) {
+  const bool alone = a.mode == kPerSegment;
+  for (int b = alone ? (int)fastdiv((uint32_t)wg, a.head_div) : wg; b < a.B;
+       b += alone ? a.B : nwg) {
     if (length_of(a, b) > 0) continue;
     for (int i = tid; i < a.Hq * kDim / 8; i += kThreads)
       reinterpret_cast<uint4*>(a.out + (size_t)b * a.Hq * kDim)[i] = make_uint4(0, 0, 0, 0);
@@ -734,32 +758,34 @@ __global__ __launch_bounds__(64 * kMergeWaves) void kv_decode_merge_kernel(Decod
   const int nh = segment_heads(a, seg, b, h0);
   const int h = (int)blockIdx.y * kMergeWaves + (threadIdx.x >> 6);
   if (h >= nh) return;
-  const size_t slot_floats = (size_t)a.heads * kPitch;
+  const uint32_t slot_floats = (uint32_t)a.heads * kPitch;
   // (Shares go to the first workgroups, so all from `from` to wg have a piece.)
-  const auto state = [&](int w) {
-    return a.states + ((size_t)w * 2 + (w == from ? 1 : 0)) * slot_floats + h * kPitch;
+  const float* const states = a.states + (size_t)from * 2 * slot_floats + h * kPitch;
+  const auto state = [&](int i) {  // piece i: a Z piece, then A pieces
+    return states + (size_t)(i ? 2 * (uint32_t)i : 1u) * slot_floats;
   };
+  const int n = wg - from + 1;
   // 32 pieces at a time: their rows and, a piece to a lane, their m and l go out
   // together with the loads of all maxima, so that up to 32 pieces take one
   // round trip.
   constexpr int kBatch = 32;
   float mloc = kNegInf, M = kNegInf;
-  for (int w = from + lane; w <= wg; w += 64) mloc = fmaxf(mloc, state(w)[kDim]);
+  for (int i = lane; i < n; i += 64) mloc = fmaxf(mloc, state(i)[kDim]);
   float L = 0.f, x = 0.f, y = 0.f;
-  for (int w0 = from; w0 <= wg; w0 += kBatch) {
+  for (int i0 = 0; i0 < n; i0 += kBatch) {
     float2 v[kBatch];
 #pragma unroll
     for (int i = 0; i < kBatch; ++i)
-      v[i] = reinterpret_cast<const float2*>(state(min(w0 + i, wg)))[lane];
+      v[i] = reinterpret_cast<const float2*>(state(min(i0 + i, n - 1)))[lane];
     const float2 ml =
-        *reinterpret_cast<const float2*>(state(min(w0 + (lane & (kBatch - 1)), wg)) + kDim);
-    if (w0 == from) M = wave_max(mloc);
+        *reinterpret_cast<const float2*>(state(min(i0 + (lane & (kBatch - 1)), n - 1)) + kDim);
+    if (i0 == 0) M = wave_max(mloc);
     const float fl = M == kNegInf ? 0.f : exp2_fast(ml.x - M);
 #pragma unroll
     for (int i = 0; i < kBatch; ++i) {
       const float f = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(fl), i));
       const float l = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(ml.y), i));
-      if (w0 + i <= wg) {
+      if (i0 + i < n) {
         L = fmaf(l, f, L);
         x = fmaf(v[i].x, f, x);
         y = fmaf(v[i].y, f, y);
@@ -771,8 +797,7 @@ __global__ __launch_bounds__(64 * kMergeWaves) void kv_decode_merge_kernel(Decod
 }
 
 struct Shape {
-  int G, chunks, heads, capacity, workgroups;
-  bool per_segment;
+  int G, chunks, heads, capacity, workgroups, mode;
 };
 
 // Longest sequence, in units, that a workgroup takes alone.
@@ -792,19 +817,20 @@ bool shape_of(int B, int Hq, int Hkv, int num_blocks, int block_size, int max_bl
   if ((int64_t)B * Hq > (int64_t(1) << 28)) return false;
   s.heads = std::min(s.G, 16);
   s.capacity = (int)cap;
-  const int64_t segments = (int64_t)B * Hkv * s.chunks;
-  s.per_segment = num_workgroups <= 0 && (cap + kUnit - 1) / kUnit <= kAloneUnits &&
-                  segments <= gqa::device_cu_count();
   s.workgroups = num_workgroups;
-  if (s.per_segment)
-    s.workgroups = (int)segments;
-  else if (num_workgroups <= 0)
+  s.mode = kBalanced;
+  if (num_workgroups <= 0) {
     s.workgroups = gqa::device_cu_count();
+    const int64_t segments = (int64_t)B * Hkv * s.chunks;
+    if ((cap + kUnit - 1) / kUnit <= kAloneUnits)
+      s.mode = segments <= s.workgroups ? kPerSegment : kWhole;
+    if (s.mode == kPerSegment) s.workgroups = (int)segments;
+  }
   return s.workgroups <= (1 << 22);
 }
 
 size_t workspace_bytes(const Shape& s) {
-  if (s.per_segment) return 0;
+  if (s.mode != kBalanced) return 0;
   return (size_t)s.workgroups * (sizeof(Record) + 2 * (size_t)s.heads * kPitch * sizeof(float));
 }
 
@@ -863,7 +889,7 @@ extern "C" int kv_decode_mxfp4_launch(const uint16_t* q, const uint8_t* mxfp4_ca
   // keeps 0 * infinity out of the kernel.)
   a.scale = std::max(fabsf(scale) * gqa::kLog2e, 1.17549435e-38f);
   a.sign = scale < 0.f ? -1.f : 1.f;
-  a.per_segment = s.per_segment;
+  a.mode = s.mode;
   const size_t lds = (size_t)kWaves * 2 * s.heads * kPitch * sizeof(float);
   const auto kernel = s.G > 8 ? kv_decode_kernel<true> : kv_decode_kernel<false>;
   if (lds > 65536) {  // more than the default share of a CU's 160 KiB
@@ -873,7 +899,7 @@ extern "C" int kv_decode_mxfp4_launch(const uint16_t* q, const uint8_t* mxfp4_ca
   }
   kernel<<<s.workgroups, kThreads, lds, stream>>>(a);
   hipError_t e = hipGetLastError();
-  if (e != hipSuccess || s.per_segment) return e;
+  if (e != hipSuccess || s.mode != kBalanced) return e;
   kv_decode_merge_kernel<<<dim3(s.workgroups, (s.heads + kMergeWaves - 1) / kMergeWaves),
                            64 * kMergeWaves, 0, stream>>>(a);
   return hipGetLastError();

@@ -460,6 +460,26 @@ def test_decode(gpu, lens, Hq, Hkv, bs):
         assert torch.equal(got, kv_cache.gqa_decode_mxfp4(*args, num_workgroups=nwg))
 
 
+@pytest.mark.parametrize("B,longest,Hq,Hkv", [(70, 900, 32, 8), (1100, 40, 8, 2), (300, 200, 20, 1),
+                                              (65, 1500, 4, 4), (513, 33, 1, 1)])
+def test_decode_many_requests(gpu, B, longest, Hq, Hkv):
+    """More requests than a wave has lanes, more than a workgroup has threads, more segments than
+    there are CUs: whole segments dealt out, and balanced shares; every seventh request empty."""
+    gen = torch.Generator().manual_seed(B)
+    S = torch.randint(1, longest + 1, (B,), generator=gen)
+    S[::7] = 0
+    S[-1], S[5] = longest, -1
+    S = S.tolist()
+    _, _, table, nb = make_step(None, S, 16, seed=B)
+    cache = poison(filled_cache(gen, nb, Hkv, 16), table, S, 16)
+    q = normal(gen, B, Hq, D)
+    args = (q.to(gpu), torch.from_numpy(cache).to(gpu), table.to(gpu), tensor(S, gpu), 0.1)
+    for nwg in (0, 256, 5):
+        got = kv_cache.gqa_decode_mxfp4(*args, num_workgroups=nwg)
+        check_attention(got, q, cache, table, S, 0.1, f"{nwg} workgroups")
+        assert torch.equal(got, kv_cache.gqa_decode_mxfp4(*args, num_workgroups=nwg))
+
+
 @pytest.mark.parametrize("scale", [0.0, -0.1, 3.0, 1e-30, 25.0])
 def test_decode_scales(gpu, scale):
     """No softmax at all (0), the smallest key first (negative), one key taking all (large)."""
