@@ -46,12 +46,15 @@ using gqa::dpp_f32;
 using gqa::exp2_fast;
 using gqa::kNegInf;
 using gqa::wave_max;
+using gqa::wave_sum;
 using gqa::xor16_max;
 using gqa::xor32_max;
 
 typedef __bf16 bf16x8_t __attribute__((ext_vector_type(8)));
 typedef float f32x2_t __attribute__((ext_vector_type(2)));
 typedef float f32x4_t __attribute__((ext_vector_type(4)));
+typedef short i16x2_t __attribute__((ext_vector_type(2)));
+typedef uint16_t u16x2_t __attribute__((ext_vector_type(2)));
 typedef int i32x8_t __attribute__((ext_vector_type(8)));
 
 constexpr int kUnit = 32;       // tokens a wave takes at a time
@@ -86,7 +89,7 @@ struct DecodeArgs {
   FastDiv tile_div;  // by tiles_per_block
   FastDiv head_div;  // by Hkv * chunks
   float scale;       // |scale| log2(e)
-  float sign;        // of scale
+  uint32_t flip;     // 0x80008000 for a negative scale: the queries change sign
   int mode;
 };
 
@@ -130,39 +133,52 @@ __device__ __forceinline__ RawQuery load_query(const DecodeArgs& a, int b, int h
   return r;
 }
 
-// The same as the B operand, in two e4m3 parts.
+__device__ __forceinline__ uint32_t xor16_umax(uint32_t x) {
+  const auto p = __builtin_amdgcn_permlane16_swap(x, x, false, false);
+  return max((uint32_t)p[0], (uint32_t)p[1]);
+}
+__device__ __forceinline__ uint32_t xor32_umax(uint32_t x) {
+  const auto p = __builtin_amdgcn_permlane32_swap(x, x, false, false);
+  return max((uint32_t)p[0], (uint32_t)p[1]);
+}
+
+// The same as the B operand, in two e4m3 parts (the conversions divide by the
+// exponent of their scale).
 template <bool kWide>
-__device__ __forceinline__ Query<kWide> split_query(const RawQuery& r, float sign, int c) {
-  float x[32];
+__device__ __forceinline__ Query<kWide> split_query(const RawQuery& r, uint32_t flip, int c) {
+  // The largest magnitude of the head, as bf16 bits.
+  u16x2_t most = {0, 0};
 #pragma unroll
   for (int part = 0; part < 4; ++part) {
-    float y[8];
-    unpack8(r.w[part], y);
+    const uint32_t w[4] = {r.w[part].x, r.w[part].y, r.w[part].z, r.w[part].w};
 #pragma unroll
-    for (int e = 0; e < 8; ++e) x[8 * part + e] = y[e] * sign;
+    for (int i = 0; i < 4; ++i)
+      most = __builtin_elementwise_max(most, __builtin_bit_cast(u16x2_t, w[i] & 0x7fff7fffu));
   }
-  float top = 0.f;
-#pragma unroll
-  for (int e = 0; e < 32; ++e) top = fmaxf(top, fabsf(x[e]));
-  top = xor32_max(xor16_max(top));
-  // E puts the largest magnitude into [128, 256); e4m3 ends at 448.
-  const int E = top > 0.f ? max((int)(__float_as_uint(top) >> 23) - 127 - 7, -118) : 0;
-  const float up = __uint_as_float((uint32_t)(127 - E) << 23);
+  uint32_t top = max((uint32_t)most.x, (uint32_t)most.y);
+  top = xor32_umax(xor16_umax(top));
+  // E puts it into [128, 256); e4m3 ends at 448. (A head that holds an infinity
+  // or NaN gets the scale NaN.)
+  const int E = max((int)(top >> 7) - 127 - 7, -118);
+  const float s = __uint_as_float((uint32_t)(127 + E) << 23);
+  const float s16 = __uint_as_float((uint32_t)(123 + E) << 23);
   Query<kWide> q;
   uint32_t hi[8], lo[8];
 #pragma unroll
   for (int w = 0; w < 8; ++w) {
-    int h = 0, r = 0;
-    const float y0 = x[4 * w] * up, y1 = x[4 * w + 1] * up;
-    const float y2 = x[4 * w + 2] * up, y3 = x[4 * w + 3] * up;
-    h = __builtin_amdgcn_cvt_pk_fp8_f32(y0, y1, h, false);
-    h = __builtin_amdgcn_cvt_pk_fp8_f32(y2, y3, h, true);
-    const f32x2_t b0 = __builtin_amdgcn_cvt_pk_f32_fp8(h, false);
-    const f32x2_t b1 = __builtin_amdgcn_cvt_pk_f32_fp8(h, true);
-    r = __builtin_amdgcn_cvt_pk_fp8_f32((y0 - b0[0]) * 16.f, (y1 - b0[1]) * 16.f, r, false);
-    r = __builtin_amdgcn_cvt_pk_fp8_f32((y2 - b1[0]) * 16.f, (y3 - b1[1]) * 16.f, r, true);
-    hi[w] = (uint32_t)h;
-    lo[w] = (uint32_t)r;
+    const uint4& four = r.w[w >> 1];
+    const uint32_t x[2] = {(w & 1 ? four.z : four.x) ^ flip, (w & 1 ? four.w : four.y) ^ flip};
+    i16x2_t h = {0, 0}, l = {0, 0};
+    h = __builtin_amdgcn_cvt_scalef32_pk_fp8_bf16(h, __builtin_bit_cast(bf16x2_t, x[0]), s, false);
+    h = __builtin_amdgcn_cvt_scalef32_pk_fp8_bf16(h, __builtin_bit_cast(bf16x2_t, x[1]), s, true);
+    hi[w] = __builtin_bit_cast(uint32_t, h);
+    const f32x2_t b0 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(hi[w], s, false);
+    const f32x2_t b1 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(hi[w], s, true);
+    l = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(l, bf16_lo(x[0]) - b0[0], bf16_hi(x[0]) - b0[1],
+                                                 s16, false);
+    l = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(l, bf16_lo(x[1]) - b1[0], bf16_hi(x[1]) - b1[1],
+                                                 s16, true);
+    lo[w] = __builtin_bit_cast(uint32_t, l);
   }
   if constexpr (kWide) {
 #pragma unroll
@@ -170,13 +186,13 @@ __device__ __forceinline__ Query<kWide> split_query(const RawQuery& r, float sig
       q.part[0][w] = (int)hi[w];
       q.part[1][w] = (int)lo[w];
     }
-    q.scale[0] = E + 127;
-    q.scale[1] = E + 123;
+    q.scale[0] = top < 0x7f80u ? E + 127 : 255;
+    q.scale[1] = top < 0x7f80u ? E + 123 : 255;
   } else {
     const bool low = c >= 8;
 #pragma unroll
     for (int w = 0; w < 8; ++w) q.part[0][w] = (int)(low ? lo[w] : hi[w]);
-    q.scale[0] = E + (low ? 123 : 127);
+    q.scale[0] = top < 0x7f80u ? E + (low ? 123 : 127) : 255;
   }
   return q;
 }
@@ -543,7 +559,7 @@ __global__ __launch_bounds__(kThreads, 2) void kv_decode_kernel(DecodeArgs a) {
   }
 
   int flags = 0, seg_a = 0, seg_z = 0;
-  const size_t slot_floats = (size_t)a.heads * kPitch;
+  const uint32_t slot_floats = (uint32_t)a.heads * kPitch;
   if (at.left > 0) {
     Walk ahead = at;
     next_unit(a, ahead, next);
@@ -563,7 +579,7 @@ __global__ __launch_bounds__(kThreads, 2) void kv_decode_kernel(DecodeArgs a) {
       }
       const int seg = at.b * Hc + at.hc, heads = nh;
       uint16_t* const out = a.out + ((size_t)at.b * a.Hq + h0) * kDim;
-      const Query<kWide> q = split_query<kWide>(raw, a.sign, c);
+      const Query<kWide> q = split_query<kWide>(raw, a.flip, c);
       at.left -= (uint32_t)k;
       if (at.left > 0) {  // the next segment's queries are on their way meanwhile
         next_segment(a, at);
@@ -647,7 +663,7 @@ __global__ __launch_bounds__(kThreads, 2) void kv_decode_kernel(DecodeArgs a) {
   // run starts inside a segment, and takes the first pieces (A) of the waves
   // after it up to the segment's end. Each head of each run is one wave's, two
   // dims a lane. Bit w of the masks is wave w's.
-  const Record m = meta[lane & (kWaves - 1)];
+  const Record m = meta[min(lane, kWaves - 1)];
   const auto bits = [&](int flag) {
     return (uint32_t)__builtin_amdgcn_ballot_w64((m.flags & flag) != 0) & ((1u << kWaves) - 1);
   };
@@ -680,34 +696,33 @@ __global__ __launch_bounds__(kThreads, 2) void kv_decode_kernel(DecodeArgs a) {
     }
     int sb, h0;
     const int nh = segment_heads(a, seg, sb, h0);
-    int h = (wave - turn) & (kWaves - 1);
+    int h = wave - turn % kWaves;
+    if (h < 0) h += kWaves;
     turn += nh;
     for (; h < nh; h += kWaves) {
-      // Piece i: wave i's A, or piece kWaves: the Z that starts the run.
-      const auto piece = [&](int i) {
-        return slots + (i == kWaves ? w * 2 + 1 : i * 2) * slot_floats + h * kPitch;
-      };
+      // Piece i: wave i's A, or piece kWaves: the Z that starts the run. A lane
+      // weighs one of them; all rows are read, those of other runs left out.
       const uint32_t live = as | (which ? 1u << kWaves : 0u);
-      float2 ml[kWaves + 1], v[kWaves + 1];
-      float M = kNegInf;
+      const auto piece = [&](int i) {
+        return slots + (uint32_t)(i == kWaves ? w * 2 + 1 : i * 2) * slot_floats + h * kPitch;
+      };
+      const int mine = min(lane, kWaves);
+      const float2 ml = *reinterpret_cast<const float2*>(piece(mine) + kDim);
+      float2 v[kWaves + 1];
 #pragma unroll
-      for (int i = 0; i <= kWaves; ++i) {
-        if (!(live >> i & 1)) continue;
-        ml[i] = *reinterpret_cast<const float2*>(piece(i) + kDim);
-        v[i] = reinterpret_cast<const float2*>(piece(i))[lane];
-      }
-#pragma unroll
-      for (int i = 0; i <= kWaves; ++i)
-        if (live >> i & 1) M = fmaxf(M, ml[i].x);
-      float L = 0.f, x = 0.f, y = 0.f;
+      for (int i = 0; i <= kWaves; ++i) v[i] = reinterpret_cast<const float2*>(piece(i))[lane];
+      const bool counts = lane <= kWaves && (live >> mine & 1);
+      const float M = wave_max(counts ? ml.x : kNegInf);
+      const float fl = counts && M != kNegInf ? exp2_fast(ml.x - M) : 0.f;
+      float L = counts ? ml.y * fl : 0.f, x = 0.f, y = 0.f;
+      L = wave_sum(L);
 #pragma unroll
       for (int j = 0; j <= kWaves; ++j) {
         const int i = j ? j - 1 : kWaves;  // in the order of the tokens
-        if (!(live >> i & 1)) continue;
-        const float f = M == kNegInf ? 0.f : exp2_fast(ml[i].x - M);
-        L = fmaf(ml[i].y, f, L);
-        x = fmaf(v[i].x, f, x);
-        y = fmaf(v[i].y, f, y);
+        const float f = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(fl), i));
+        const bool in = live >> i & 1;
+        x = fmaf(in ? v[i].x : 0.f, f, x);
+        y = fmaf(in ? v[i].y : 0.f, f, y);
       }
       if (to_out) {
         reinterpret_cast<uint32_t*>(a.out + ((size_t)sb * a.Hq + h0 + h) * kDim)[lane] =
@@ -888,7 +903,7 @@ extern "C" int kv_decode_mxfp4_launch(const uint16_t* q, const uint8_t* mxfp4_ca
   // (A scale of 0 weighs all tokens alike; the smallest normal does as well and
   // keeps 0 * infinity out of the kernel.)
   a.scale = std::max(fabsf(scale) * gqa::kLog2e, 1.17549435e-38f);
-  a.sign = scale < 0.f ? -1.f : 1.f;
+  a.flip = scale < 0.f ? 0x80008000u : 0u;
   a.mode = s.mode;
   const size_t lds = (size_t)kWaves * 2 * s.heads * kPitch * sizeof(float);
   const auto kernel = s.G > 8 ? kv_decode_kernel<true> : kv_decode_kernel<false>;

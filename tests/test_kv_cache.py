@@ -535,6 +535,22 @@ def test_decode_nan_and_infinite_keys_stay_in_their_head(gpu):
     assert torch.isfinite(got).all()
 
 
+def test_decode_queries_that_are_not_finite(gpu):
+    """An infinity or NaN in a query gives its head NaN, and no other head."""
+    S, Hkv, bs = [40, 70], 2, 16
+    gen = torch.Generator().manual_seed(11)
+    _, B, table, nb = make_step(None, S, bs, seed=2)
+    cache = filled_cache(gen, nb, Hkv, bs)
+    for Hq in (8, 24):
+        q = normal(gen, B, Hq, D)
+        q[0, 1, 77], q[1, 0, 3], q[1, Hq - 1, 127] = math.nan, math.inf, -math.inf
+        got = kv_cache.gqa_decode_mxfp4(q.to(gpu), torch.from_numpy(cache).to(gpu), table.to(gpu),
+                                        tensor(S, gpu), 0.1)
+        bad = torch.zeros(B, Hq, dtype=torch.bool, device=gpu)
+        bad[0, 1] = bad[1, 0] = bad[1, Hq - 1] = True
+        assert torch.isnan(got[bad]).all() and torch.isfinite(got[~bad]).all()
+
+
 def test_decode_empty_batch_and_unaligned_q(gpu):
     cache = kv_cache.new_mxfp4_cache(4, 16, 2)
     out = kv_cache.gqa_decode_mxfp4(torch.zeros(0, 8, D, dtype=torch.bfloat16, device=gpu), cache,
