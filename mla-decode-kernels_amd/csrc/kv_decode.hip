@@ -378,8 +378,12 @@ __device__ __forceinline__ void fold_unit(const Unit& u, const Mask& mask, const
   two_dims(std::integral_constant<int, 3>{});
 }
 
-// out = acc / l; a segment without a single token gets zeros.
-__device__ __forceinline__ float normal(float acc, float l) { return l == 0.f ? 0.f : acc / l; }
+// What a row is multiplied by in the end, 1 / l; a segment without a single token
+// gets zeros. (One quotient a lane: its fp32 rounding is nothing to bf16's.)
+__device__ __forceinline__ float inverse(float l) { return l == 0.f ? 0.f : 1.f / l; }
+__device__ __forceinline__ uint32_t pack2(float x, float y) {
+  return f32_to_bf16_bits(x) | (f32_to_bf16_bits(y) << 16);
+}
 
 // The q-heads of segment (b, hc): h0 .. h0 + the result - 1.
 __device__ __forceinline__ int heads_of(const DecodeArgs& a, int hc, int& h0) {
@@ -621,11 +625,12 @@ __global__ __launch_bounds__(kThreads, 2) void kv_decode_kernel(DecodeArgs a) {
       if (starts && ends) {
         if (c < heads) {
           uint16_t* dst = out + c * kDim + 32 * g;
+          const float r = inverse(l);
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
             float y[8];
 #pragma unroll
-            for (int j = 0; j < 8; ++j) y[j] = normal(st.o[j][e], l);
+            for (int j = 0; j < 8; ++j) y[j] = st.o[j][e] * r;
             *reinterpret_cast<uint4*>(dst + 8 * e) = pack8(y);
           }
         }
@@ -726,7 +731,7 @@ __global__ __launch_bounds__(kThreads, 2) void kv_decode_kernel(DecodeArgs a) {
       }
       if (to_out) {
         reinterpret_cast<uint32_t*>(a.out + ((size_t)sb * a.Hq + h0 + h) * kDim)[lane] =
-            f32_to_bf16_bits(normal(x, L)) | (f32_to_bf16_bits(normal(y, L)) << 16);
+            pack2(x * inverse(L), y * inverse(L));
       } else {
         float* dst = a.states + ((size_t)wg * 2 + which) * slot_floats + h * kPitch;
         reinterpret_cast<float2*>(dst)[lane] = make_float2(x, y);
@@ -808,7 +813,7 @@ __global__ __launch_bounds__(64 * kMergeWaves) void kv_decode_merge_kernel(Decod
     }
   }
   reinterpret_cast<uint32_t*>(a.out + ((size_t)b * a.Hq + h0 + h) * kDim)[lane] =
-      f32_to_bf16_bits(normal(x, L)) | (f32_to_bf16_bits(normal(y, L)) << 16);
+      pack2(x * inverse(L), y * inverse(L));
 }
 
 struct Shape {
