@@ -24,9 +24,14 @@ constexpr int kWaves = 4;  // waves of a workgroup: neighbouring head ranges of 
 // other element, the sign of its sine in s.
 struct Turn {
   float c[8], s[8];
-  int partner;  // the lane (of the wave) that holds x', -1: this one (interleaved pairs)
+  int partner;  // the lane (of the wave) that holds x'
   bool on;      // these dims rotate
 };
+
+// How pairs lie: neighbours in a lane, 8 lanes apart (the halves of 128 dims: a
+// rotation by 8 within the DPP row, no LDS), or in lane `partner`.
+enum Pairs { kInside, kHalfRow, kPartner };
+
 
 // kLanes lanes hold a row of 8 kLanes dims, of which the first rot turn.
 template <int kLanes>
@@ -69,12 +74,23 @@ __device__ __forceinline__ Turn load_turn(const float* __restrict__ cos_sin, int
   return t;
 }
 
+__device__ __forceinline__ float half_row(float x) { return dpp_f32<0x128>(x); }
+__device__ __forceinline__ double half_row(double x) {
+  const uint64_t u = __builtin_bit_cast(uint64_t, x);
+  const uint32_t lo = __builtin_amdgcn_update_dpp(0, (int)(uint32_t)u, 0x128, 0xF, 0xF, true);
+  const uint32_t hi = __builtin_amdgcn_update_dpp(0, (int)(u >> 32), 0x128, 0xF, 0xF, true);
+  return __builtin_bit_cast(double, (uint64_t)lo | ((uint64_t)hi << 32));
+}
+
 // The pair's other elements of x (every lane of the wave calls this).
 template <class F>
-__device__ __forceinline__ void others(const F (&x)[8], F (&y)[8], const Turn& t, bool interleaved) {
-  if (interleaved) {
+__device__ __forceinline__ void others(const F (&x)[8], F (&y)[8], const Turn& t, Pairs pairs) {
+  if (pairs == kInside) {
 #pragma unroll
     for (int e = 0; e < 8; ++e) y[e] = x[e ^ 1];
+  } else if (pairs == kHalfRow) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) y[e] = half_row(x[e]);
   } else {
 #pragma unroll
     for (int e = 0; e < 8; ++e) y[e] = __shfl(x[e], t.partner, 64);
@@ -82,19 +98,19 @@ __device__ __forceinline__ void others(const F (&x)[8], F (&y)[8], const Turn& t
 }
 
 // Norm over the head's 128 dims (16 lanes), then the rotation.
-__device__ __forceinline__ void norm_turn(float (&x)[8], const float* w, float eps, const Turn& t,
-                                          bool rotate, bool interleaved) {
-  if (w) {
+__device__ __forceinline__ void norm_turn(float (&x)[8], bool norm, const float (&w)[8], float eps,
+                                          const Turn& t, bool rotate, Pairs pairs) {
+  if (norm) {
     float ss = 0.f;
 #pragma unroll
     for (int e = 0; e < 8; ++e) ss = fmaf(x[e], x[e], ss);
-    const float r = 1.f / sqrtf(row16_sum(ss) * (1.f / kDim) + eps);
+    const float r = rsqrtf(row16_sum(ss) * (1.f / kDim) + eps);
 #pragma unroll
     for (int e = 0; e < 8; ++e) x[e] = x[e] * r * w[e];
   }
   if (!rotate) return;
   float y[8];
-  others(x, y, t, interleaved);
+  others(x, y, t, pairs);
   if (!t.on) return;
 #pragma unroll
   for (int e = 0; e < 8; ++e) x[e] = fmaf(x[e], t.c[e], y[e] * t.s[e]);
@@ -104,12 +120,12 @@ __device__ __forceinline__ void norm_turn(float (&x)[8], const float* w, float e
 // products are exact, the sum of 128 squares nearly, and what is left is off by
 // 2^-50, far less than the chance distance to a border between two codes.
 // (gfx950 runs fp64 FMAs at the rate of fp32 ones.)
-__device__ __forceinline__ void norm_turn64(float (&x)[8], const float* w, float eps,
-                                            const Turn& t, bool rotate, bool interleaved) {
+__device__ __forceinline__ void norm_turn64(float (&x)[8], bool norm, const float (&w)[8],
+                                            float eps, const Turn& t, bool rotate, Pairs pairs) {
   double d[8];
 #pragma unroll
   for (int e = 0; e < 8; ++e) d[e] = x[e];
-  if (w) {
+  if (norm) {
     double ss = 0.;
 #pragma unroll
     for (int e = 0; e < 8; ++e) ss = fma(d[e], d[e], ss);
@@ -121,7 +137,7 @@ __device__ __forceinline__ void norm_turn64(float (&x)[8], const float* w, float
   }
   if (rotate) {
     double y[8];
-    others(d, y, t, interleaved);
+    others(d, y, t, pairs);
     if (t.on) {
 #pragma unroll
       for (int e = 0; e < 8; ++e) d[e] = fma(d[e], (double)t.c[e], y[e] * (double)t.s[e]);
@@ -156,10 +172,14 @@ __device__ __forceinline__ uint32_t encode8(const float (&x)[8], uint32_t& scale
   return c;
 }
 
-__device__ __forceinline__ float weight_at(const void* w, int type, int d) {
-  return type == KV_WEIGHT_FP32
-             ? static_cast<const float*>(w)[d]
-             : __uint_as_float((uint32_t) static_cast<const uint16_t*>(w)[d] << 16);
+// Weights d .. d + 7.
+__device__ __forceinline__ void load_weights(const void* p, int type, int d, float (&w)[8]) {
+  if (type == KV_WEIGHT_FP32) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) w[e] = static_cast<const float*>(p)[d + e];
+  } else {
+    unpack8(load16(static_cast<const uint16_t*>(p) + d), w);
+  }
 }
 
 // Grid: x groups of four tokens, y ranges of kWaves * R rows (q heads, then k
@@ -191,12 +211,15 @@ __global__ __launch_bounds__(64 * kWaves) void kv_append_kernel(kv_append_args a
   const Place place = find_place<16>(t, a.T, a.B, a.seq_lens, a.cu_seqlens, lane);
   int slot;
   const int block = find_block(place, a.block_table, a.max_blocks, a.num_blocks, bs_div, slot);
-  const bool rotate = a.rotary_dim > 0, inter = a.interleaved != 0;
+  const bool rotate = a.rotary_dim > 0;
+  const Pairs pairs = a.interleaved ? kInside : a.rotary_dim == kDim ? kHalfRow : kPartner;
   Turn turn{};
   if (rotate && r0 < a.Hq + a.Hkv)
     turn = load_turn<16>(a.cos_sin, a.table_rows, a.rotary_dim, a.interleaved,
                          a.rope_positions && in ? a.rope_positions[t] : place.pos, lane);
 
+  float w[8] = {};
+  const void* have = nullptr;  // whose weights w holds
 #pragma unroll
   for (int j = 0; j < R; ++j) {
     const int r = r0 + j;
@@ -206,16 +229,14 @@ __global__ __launch_bounds__(64 * kWaves) void kv_append_kernel(kv_append_args a
     unpack8(raw[j], x);
     if (is_q || is_k) {
       const void* wp = is_q ? a.q_weight : a.k_weight;
-      float w[8];
-      if (wp) {
-        const int type = is_q ? a.q_weight_type : a.k_weight_type;
-#pragma unroll
-        for (int e = 0; e < 8; ++e) w[e] = weight_at(wp, type, 8 * i + e);
+      if (wp && wp != have) {
+        load_weights(wp, is_q ? a.q_weight_type : a.k_weight_type, 8 * i, w);
+        have = wp;
       }
       if (kMx && is_k)
-        norm_turn64(x, wp ? w : nullptr, a.eps, turn, rotate, inter);
+        norm_turn64(x, wp != nullptr, w, a.eps, turn, rotate, pairs);
       else
-        norm_turn(x, wp ? w : nullptr, a.eps, turn, rotate, inter);
+        norm_turn(x, wp != nullptr, w, a.eps, turn, rotate, pairs);
     }
     if (is_q) {
       if (in)
@@ -319,10 +340,11 @@ __global__ __launch_bounds__(64 * kWaves) void kv_append_mla_kernel(kv_append_ml
       float ss = 0.f;
 #pragma unroll
       for (int e = 0; e < 8; ++e) ss = fmaf(x[e], x[e], ss);
-      const float r = 1.f / sqrtf(gqa::wave_sum(ss) * (1.f / kLatent) + a.eps);
+      const float r = rsqrtf(gqa::wave_sum(ss) * (1.f / kLatent) + a.eps);
+      float w[8];
+      load_weights(a.c_weight, a.c_weight_type, 8 * lane, w);
 #pragma unroll
-      for (int e = 0; e < 8; ++e)
-        x[e] = x[e] * r * weight_at(a.c_weight, a.c_weight_type, 8 * lane + e);
+      for (int e = 0; e < 8; ++e) x[e] = x[e] * r * w[e];
       raw = pack8(x);
     }
     if (block >= 0) *reinterpret_cast<uint4*>(dst + 8 * lane) = raw;
@@ -331,7 +353,7 @@ __global__ __launch_bounds__(64 * kWaves) void kv_append_mla_kernel(kv_append_ml
   const Turn turn = load_turn<8>(a.cos_sin, a.table_rows, kRope, a.interleaved,
                                  a.rope_positions ? a.rope_positions[t] : place.pos, lane);
   float y[8];
-  others(x, y, turn, a.interleaved != 0);
+  others(x, y, turn, a.interleaved ? kInside : kPartner);
 #pragma unroll
   for (int e = 0; e < 8; ++e) x[e] = fmaf(x[e], turn.c[e], y[e] * turn.s[e]);
   if (is_q)

@@ -12,7 +12,6 @@ namespace kv {
 
 using gqa::bf16_hi;
 using gqa::bf16_lo;
-using gqa::f32_to_bf16_bits;
 using gqa::FastDiv;
 using gqa::fastdiv;
 using gqa::make_fastdiv;
@@ -58,13 +57,14 @@ __device__ __forceinline__ void unpack8(const uint4& w, float (&x)[8]) {
   x[0] = bf16_lo(w.x); x[1] = bf16_hi(w.x); x[2] = bf16_lo(w.y); x[3] = bf16_hi(w.y);
   x[4] = bf16_lo(w.z); x[5] = bf16_hi(w.z); x[6] = bf16_lo(w.w); x[7] = bf16_hi(w.w);
 }
-// Round to nearest even, once: the only rounding of a bf16 append.
+// Two fp32 values as bf16, to nearest even (v_cvt_pk_bf16_f32).
+typedef float f32x2_t __attribute__((ext_vector_type(2)));
+__device__ __forceinline__ uint32_t pack2(float x, float y) {
+  return __builtin_bit_cast(uint32_t, __builtin_convertvector(f32x2_t{x, y}, bf16x2_t));
+}
+// The only rounding of a bf16 append.
 __device__ __forceinline__ uint4 pack8(const float (&x)[8]) {
-  uint32_t w[4];
-#pragma unroll
-  for (int i = 0; i < 4; ++i)
-    w[i] = f32_to_bf16_bits(x[2 * i]) | (f32_to_bf16_bits(x[2 * i + 1]) << 16);
-  return make_uint4(w[0], w[1], w[2], w[3]);
+  return make_uint4(pack2(x[0], x[1]), pack2(x[2], x[3]), pack2(x[4], x[5]), pack2(x[6], x[7]));
 }
 
 // fp64 -> fp32 rounded to odd: truncated, with the last bit set if anything was

@@ -51,7 +51,6 @@ using gqa::xor16_max;
 using gqa::xor32_max;
 
 typedef __bf16 bf16x8_t __attribute__((ext_vector_type(8)));
-typedef float f32x2_t __attribute__((ext_vector_type(2)));
 typedef float f32x4_t __attribute__((ext_vector_type(4)));
 typedef short i16x2_t __attribute__((ext_vector_type(2)));
 typedef uint16_t u16x2_t __attribute__((ext_vector_type(2)));
@@ -381,9 +380,6 @@ __device__ __forceinline__ void fold_unit(const Unit& u, const Mask& mask, const
 // What a row is multiplied by in the end, 1 / l; a segment without a single token
 // gets zeros. (One quotient a lane: its fp32 rounding is nothing to bf16's.)
 __device__ __forceinline__ float inverse(float l) { return l == 0.f ? 0.f : 1.f / l; }
-__device__ __forceinline__ uint32_t pack2(float x, float y) {
-  return f32_to_bf16_bits(x) | (f32_to_bf16_bits(y) << 16);
-}
 
 // The q-heads of segment (b, hc): h0 .. h0 + the result - 1.
 __device__ __forceinline__ int heads_of(const DecodeArgs& a, int hc, int& h0) {
