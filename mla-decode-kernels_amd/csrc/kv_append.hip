@@ -8,6 +8,8 @@
 // and their angles (16 registers) are found once and serve every head. In
 // the 4-bit cache four tokens of a request, if they are aligned, are one whole
 // 256-byte line of value codes.
+#include <type_traits>
+
 #include "kv_cache.h"
 
 #include "kv_common.hpp"
@@ -182,85 +184,113 @@ __device__ __forceinline__ void load_weights(const void* p, int type, int d, flo
   }
 }
 
-// Grid: x groups of four tokens, y ranges of kWaves * R rows (q heads, then k
-// heads, then v heads); a wave takes R of them.
+// Store 8 dims of one key or value row of the 4-bit cache. All lanes of a quad
+// call it (they exchange their maxima).
+__device__ __forceinline__ void store_mx(const kv_append_args& a, int block, int slot, int head,
+                                         int i, bool key, const float (&x)[8]) {
+  uint32_t scale;
+  const uint32_t code = encode8(x, scale);
+  if (block < 0) return;
+  uint8_t* tile = a.mxfp4_cache + (((size_t)block * a.Hkv + head) * (a.block_size / kTileTokens) +
+                                   slot / kTileTokens) * kTileBytes;
+  const int s = slot % kTileTokens;
+  *reinterpret_cast<uint32_t*>(tile + (key ? key_code_at(s, i) : value_code_at(s, i))) = code;
+  if ((i & 3) == 0)
+    tile[key ? key_scale_at(s, i >> 2) : value_scale_at(s, i >> 2)] = (uint8_t)scale;
+}
+
+// Heads a wave takes: R of the queries, of the values, and of the keys of the
+// bf16 cache; one of the keys of the 4-bit cache, whose fp64 arithmetic on
+// several rows at once would take the registers of half the waves (append and
+// read-back of 3880 tokens: 37 us at 4 keys a wave, 32 us at 1).
+template <bool kMx, int R>
+struct Tasks {
+  static constexpr int kKeys = kMx ? 1 : R;
+  int q, k, v;
+  __host__ __device__ Tasks(int Hq, int Hkv)
+      : q((Hq + R - 1) / R), k((Hkv + kKeys - 1) / kKeys), v((Hkv + R - 1) / R) {}
+};
+
+// Grid: x groups of four tokens, y groups of kWaves tasks (queries, then keys, then
+// values).
 template <bool kMx, int R>
 __global__ __launch_bounds__(64 * kWaves) void kv_append_kernel(kv_append_args a, FastDiv bs_div) {
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int lane = threadIdx.x & 63;
   const int i = lane & 15;
   const int t = (int)blockIdx.x * 4 + (lane >> 4);
-  const int rows = a.Hq + 2 * a.Hkv;
-  const int r0 = ((int)blockIdx.y * kWaves + wave) * R;
-  if (r0 >= rows) return;
+  const Tasks<kMx, R> tasks(a.Hq, a.Hkv);
+  const int task = (int)blockIdx.y * kWaves + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  if (task >= tasks.q + tasks.k + tasks.v) return;
+  const bool is_q = task < tasks.q, is_k = !is_q && task < tasks.q + tasks.k;
+  const int h0 = is_q ? task * R
+                 : is_k ? (task - tasks.q) * tasks.kKeys
+                        : (task - tasks.q - tasks.k) * R;
+  const int n = min(is_k ? tasks.kKeys : R, (is_q ? a.Hq : a.Hkv) - h0);
   const bool in = t < a.T;
 
   // The rows' loads go out first: they need no place.
+  const uint16_t* const src = is_q ? a.q : is_k ? a.k : a.v;
+  const int64_t st = is_q ? a.q_token_stride : is_k ? a.k_token_stride : a.v_token_stride;
+  const int64_t sh = is_q ? a.q_head_stride : is_k ? a.k_head_stride : a.v_head_stride;
   uint4 raw[R];
 #pragma unroll
   for (int j = 0; j < R; ++j) {
     raw[j] = make_uint4(0, 0, 0, 0);
-    const int r = r0 + j;
-    if (!in || r >= rows) continue;
-    const uint16_t* p = r < a.Hq ? a.q + t * a.q_token_stride + r * a.q_head_stride
-                        : r < a.Hq + a.Hkv
-                            ? a.k + t * a.k_token_stride + (r - a.Hq) * a.k_head_stride
-                            : a.v + t * a.v_token_stride + (r - a.Hq - a.Hkv) * a.v_head_stride;
-    raw[j] = load16(p + 8 * i);
+    if (in && j < n) raw[j] = load16(src + t * st + (h0 + j) * sh + 8 * i);
   }
 
   const Place place = find_place<16>(t, a.T, a.B, a.seq_lens, a.cu_seqlens, lane);
   int slot;
   const int block = find_block(place, a.block_table, a.max_blocks, a.num_blocks, bs_div, slot);
+
+  if (!is_q && !is_k) {
+#pragma unroll
+    for (int j = 0; j < R; ++j) {
+      if (j >= n) break;
+      if constexpr (kMx) {
+        float x[8];
+        unpack8(raw[j], x);
+        store_mx(a, block, slot, h0 + j, i, false, x);
+      } else if (block >= 0) {
+        *reinterpret_cast<uint4*>(
+            a.v_cache + (((size_t)block * a.block_size + slot) * a.Hkv + h0 + j) * kDim + 8 * i) =
+            raw[j];
+      }
+    }
+    return;
+  }
+
   const bool rotate = a.rotary_dim > 0;
   const Pairs pairs = a.interleaved ? kInside : a.rotary_dim == kDim ? kHalfRow : kPartner;
   Turn turn{};
-  if (rotate && r0 < a.Hq + a.Hkv)
+  if (rotate)
     turn = load_turn<16>(a.cos_sin, a.table_rows, a.rotary_dim, a.interleaved,
                          a.rope_positions && in ? a.rope_positions[t] : place.pos, lane);
-
+  const void* const weight = is_q ? a.q_weight : a.k_weight;
   float w[8] = {};
-  const void* have = nullptr;  // whose weights w holds
+  if (weight) load_weights(weight, is_q ? a.q_weight_type : a.k_weight_type, 8 * i, w);
+
+  if (kMx && is_k) {
+    float x[8];
+    unpack8(raw[0], x);
+    norm_turn64(x, weight != nullptr, w, a.eps, turn, rotate, pairs);
+    store_mx(a, block, slot, h0, i, true, x);
+    return;
+  }
 #pragma unroll
   for (int j = 0; j < R; ++j) {
-    const int r = r0 + j;
-    if (r >= rows) break;
-    const bool is_q = r < a.Hq, is_k = !is_q && r < a.Hq + a.Hkv;
+    if (j >= n) break;
     float x[8];
     unpack8(raw[j], x);
-    if (is_q || is_k) {
-      const void* wp = is_q ? a.q_weight : a.k_weight;
-      if (wp && wp != have) {
-        load_weights(wp, is_q ? a.q_weight_type : a.k_weight_type, 8 * i, w);
-        have = wp;
-      }
-      if (kMx && is_k)
-        norm_turn64(x, wp != nullptr, w, a.eps, turn, rotate, pairs);
-      else
-        norm_turn(x, wp != nullptr, w, a.eps, turn, rotate, pairs);
-    }
+    norm_turn(x, weight != nullptr, w, a.eps, turn, rotate, pairs);
     if (is_q) {
       if (in)
-        store16(a.q_out + t * a.q_out_token_stride + r * a.q_out_head_stride + 8 * i,
+        store16(a.q_out + t * a.q_out_token_stride + (h0 + j) * a.q_out_head_stride + 8 * i,
                 place.live ? pack8(x) : make_uint4(0, 0, 0, 0));
-      continue;
-    }
-    const int head = is_k ? r - a.Hq : r - a.Hq - a.Hkv;
-    if constexpr (kMx) {
-      uint32_t scale;
-      const uint32_t code = encode8(x, scale);  // (all lanes: quads exchange maxima)
-      if (block >= 0) {
-        uint8_t* tile = a.mxfp4_cache +
-                        (((size_t)block * a.Hkv + head) * (a.block_size / kTileTokens) +
-                         slot / kTileTokens) * kTileBytes;
-        const int s = slot % kTileTokens;
-        *reinterpret_cast<uint32_t*>(tile + (is_k ? key_code_at(s, i) : value_code_at(s, i))) =
-            code;
-        if ((i & 3) == 0)
-          tile[is_k ? key_scale_at(s, i >> 2) : value_scale_at(s, i >> 2)] = (uint8_t)scale;
-      }
     } else if (block >= 0) {
-      const size_t at = (((size_t)block * a.block_size + slot) * a.Hkv + head) * kDim + 8 * i;
-      *reinterpret_cast<uint4*>((is_k ? a.k_cache : a.v_cache) + at) = is_k ? pack8(x) : raw[j];
+      *reinterpret_cast<uint4*>(
+          a.k_cache + (((size_t)block * a.block_size + slot) * a.Hkv + h0 + j) * kDim + 8 * i) =
+          pack8(x);
     }
   }
 }
@@ -408,13 +438,20 @@ int append(const kv_append_args* args, hipStream_t stream) {
   if (e != hipSuccess) return e;
   if (args->T == 0) return hipSuccess;
   const kv_append_args a = *args;
-  const int rows = a.Hq + 2 * a.Hkv;
-  const unsigned tokens = (unsigned)((a.T + 3) / 4);
-  const auto grid = [&](int R) { return dim3(tokens, (rows + kWaves * R - 1) / (kWaves * R)); };
-  if ((int64_t)tokens * rows <= 16384)
-    kv_append_kernel<kMx, 1><<<grid(1), 64 * kWaves, 0, stream>>>(a, make_fastdiv(a.block_size));
+  const unsigned groups = (unsigned)((a.T + 3) / 4);
+  const FastDiv bs_div = make_fastdiv((uint32_t)a.block_size);
+  const auto launch = [&](auto few) {
+    constexpr int R = decltype(few)::value;
+    const Tasks<kMx, R> tasks(a.Hq, a.Hkv);
+    kv_append_kernel<kMx, R>
+        <<<dim3(groups, (tasks.q + tasks.k + tasks.v + kWaves - 1) / kWaves), 64 * kWaves, 0,
+           stream>>>(a, bs_div);
+  };
+  // One head a wave until that makes 16 waves for every SIMD of 256 CUs, then 4.
+  if ((int64_t)groups * (a.Hq + 2 * a.Hkv) <= 16384)
+    launch(std::integral_constant<int, 1>{});
   else
-    kv_append_kernel<kMx, 4><<<grid(4), 64 * kWaves, 0, stream>>>(a, make_fastdiv(a.block_size));
+    launch(std::integral_constant<int, 4>{});
   return hipGetLastError();
 }
 
