@@ -463,14 +463,17 @@ __global__ __launch_bounds__(kThreads, 2) void kv_decode_kernel(DecodeArgs a) {
   Spot next{};
   Unit x0, x1;
   RawQuery raw;
+  int h0 = 0, nh = 0;  // the q-heads of the segment that raw holds
   if (a.mode == kPerSegment) {
     at.b = (int)fastdiv((uint32_t)wg, a.head_div);
     at.hc = wg - at.b * Hc;
     at.u = wave;
     at.step = kWaves;
-    // The first unit is loaded before its length is known (the table row is there
-    // to its end, and an id is looked at before it is used): one memory latency
-    // less in a launch that has little else.
+    // The queries and the first unit are loaded before the length is known (the
+    // table row is there to its end, and an id is looked at before it is used):
+    // one memory latency less in a launch that has little else.
+    nh = heads_of(a, at.hc, h0);
+    raw = load_query<kWide>(a, at.b, h0, nh, c, g);
     if (wave < units_of(a.capacity)) {
       next = find_unit(a, table_of(a, at.b), at.hc / a.chunks, a.capacity, wave);
       load_unit(a, next, lane, x0);
@@ -563,10 +566,13 @@ __global__ __launch_bounds__(kThreads, 2) void kv_decode_kernel(DecodeArgs a) {
   if (at.left > 0) {
     Walk ahead = at;
     next_unit(a, ahead, next);
-    if (a.mode != kPerSegment) load_unit(a, next, lane, x0);
+    if (a.mode != kPerSegment) {
+      // (The queries first: their conversion waits for no tile.)
+      nh = heads_of(a, at.hc, h0);
+      raw = load_query<kWide>(a, at.b, h0, nh, c, g);
+      load_unit(a, next, lane, x0);
+    }
     next_unit(a, ahead, next);
-    int h0, nh = heads_of(a, at.hc, h0);
-    raw = load_query<kWide>(a, at.b, h0, nh, c, g);
     Mask mask;
     bool unmasked = false;
     while (true) {
