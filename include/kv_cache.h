@@ -170,7 +170,7 @@ GQA_DECODE_API int kv_append_mla_launch(const kv_append_mla_args* args, hipStrea
  * request of length 0 gets zeros. Tokens in blocks whose id is outside
  * [0, num_blocks) are left out (a request with no other token gets zeros).
  * B * ceil(max_blocks * block_size / 32) * Hkv * ceil(Hq / Hkv / 16) is at most
- * 2^31 - 1.
+ * 2^31 - 1, and so are the bytes of a block (of all heads).
  *
  * Token-balanced: a grid of num_workgroups workgroups (<= 0: chosen from the
  * sizes and the current device), each taking an equal share of the batch's

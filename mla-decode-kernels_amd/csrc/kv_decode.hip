@@ -85,6 +85,7 @@ struct DecodeArgs {
   Record* records;   // [workgroups]
   int B, Hq, Hkv, G, chunks, heads;  // heads: the largest number of q-heads of a segment
   int num_blocks, tiles_per_block, max_blocks, capacity;
+  uint32_t head_bytes, block_bytes;  // of one head's tiles in a block, of all heads'
   FastDiv tile_div;  // by tiles_per_block
   FastDiv head_div;  // by Hkv * chunks
   float scale;       // |scale| log2(e)
@@ -96,7 +97,8 @@ struct DecodeArgs {
 struct Unit {
   uint4 k[2], v[2];
   uint32_t ks[2], vs[2];
-  int valid[2];  // tokens of each tile that count (0 .. 16)
+  int rest;     // tokens from its first one to the sequence's end
+  uint32_t ok;  // bit h: tile h lies in the cache
 };
 
 template <bool kWide>
@@ -205,46 +207,60 @@ typedef const __attribute__((address_space(4))) int* const_ints;
 // hides behind a fold.
 struct Spot {
   int id[2];
-  uint32_t tile[2];  // the tile's number in a block of all heads' tiles
-  int valid[2];      // tokens of each tile that are below the length (0 .. 16)
+  uint32_t off[2];  // the tile's bytes in its block
+  int rest;
 };
 
-__device__ __forceinline__ Spot find_unit(const DecodeArgs& a, const_ints table, int head, int len,
-                                          int u) {
+// The segment a walk is in: its table row and the head's place in a block.
+struct Segment {
+  const_ints table;
+  uint32_t head_off;
+  int len;
+};
+
+__device__ __forceinline__ Segment segment_of(const DecodeArgs& a, int b, int hc, int len) {
+  return Segment{(const_ints)(a.block_table + (size_t)b * a.max_blocks),
+                 (uint32_t)(hc / a.chunks) * a.head_bytes, len};
+}
+
+__device__ __forceinline__ Spot find_unit(const DecodeArgs& a, const Segment& seg, int u) {
   Spot s;
-#pragma unroll
-  for (int h = 0; h < 2; ++h) {
-    // (A second tile past the end: the first one once more, no token of it.)
-    const int first = u * kUnit + h * kTileTokens;
-    s.valid[h] = min(max(len - first, 0), kTileTokens);
-    const uint32_t t = 2 * (uint32_t)u + (s.valid[h] > 0 ? h : 0);
-    const uint32_t lb = fastdiv(t, a.tile_div);
-    s.id[h] = table[lb];
-    s.tile[h] = (uint32_t)head * a.tiles_per_block + (t - lb * a.tile_div.d);
-  }
+  s.rest = seg.len - u * kUnit;
+  uint32_t lb = fastdiv(2 * (uint32_t)u, a.tile_div);
+  uint32_t t = 2 * (uint32_t)u - lb * a.tile_div.d;
+  s.id[0] = seg.table[lb];
+  s.off[0] = seg.head_off + t * kTileBytes;
+  // (A second tile past the end: the first one once more, no token of it.)
+  if (s.rest > kTileTokens && ++t == a.tile_div.d) t = 0, ++lb;
+  s.id[1] = seg.table[lb];
+  s.off[1] = seg.head_off + t * kTileBytes;
   return s;
 }
 
-__device__ __forceinline__ uint4 stream16(const uint8_t* p) {
-  const u32x4 v = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(p));
-  return make_uint4(v.x, v.y, v.z, v.w);
-}
+// Loads through a buffer resource that covers one tile: a scalar base, fixed
+// 32-bit lane offsets, no address arithmetic in vector registers. 2: streamed
+// (nt), each byte is read once.
+struct Lanes {
+  uint32_t codes, ks, vs;  // byte offsets in each part of a tile
+};
 
-__device__ __forceinline__ void load_unit(const DecodeArgs& a, const Spot& s, uint32_t lane,
+__device__ __forceinline__ void load_unit(const DecodeArgs& a, const Spot& s, const Lanes& at,
                                           Unit& u) {
+  u.rest = s.rest;
+  u.ok = 0;
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
     // An id outside the cache: block 0 is read, no token of it counts.
     const bool in = (uint32_t)s.id[h] < (uint32_t)a.num_blocks;
-    u.valid[h] = in ? s.valid[h] : 0;
-    const uint8_t* p =
-        a.cache + ((size_t)(in ? s.id[h] : 0) * ((uint32_t)a.Hkv * a.tiles_per_block) + s.tile[h]) *
-                      kTileBytes;
-    u.k[h] = stream16(p + 16 * lane);
-    u.v[h] = stream16(p + kValueCodes + 16 * lane);
-    u.ks[h] = p[kKeyScales + lane];
-    u.vs[h] = *reinterpret_cast<const uint32_t*>(p + kValueScales + (lane >> 4) * 16 +
-                                                 ((lane & 15) >> 2) * 4);
+    u.ok |= in ? 1u << h : 0u;
+    const uint8_t* p = a.cache + (uint64_t)(in ? (uint32_t)s.id[h] : 0u) * a.block_bytes + s.off[h];
+    const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc(
+        const_cast<uint8_t*>(p), 0, kTileBytes, 0x00020000);
+    u.k[h] = __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(r, at.codes, 0, 2));
+    u.v[h] = __builtin_bit_cast(
+        uint4, __builtin_amdgcn_raw_buffer_load_b128(r, at.codes + kValueCodes, 0, 2));
+    u.ks[h] = __builtin_amdgcn_raw_buffer_load_b8(r, at.ks + kKeyScales, 0, 0);
+    u.vs[h] = __builtin_amdgcn_raw_buffer_load_b32(r, at.vs + kValueScales, 0, 0);
   }
 }
 
@@ -257,14 +273,15 @@ struct Mask {
   uint32_t ks[2], vs[2];
 };
 
-__device__ __forceinline__ void set_mask(Mask& m, const int (&valid)[2], int c, int g) {
+__device__ __forceinline__ void set_mask(Mask& m, int rest, uint32_t ok, int c, int g) {
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
-    m.ks[h] = c < valid[h] ? 0xffu : 0u;
+    const int valid = ok >> h & 1 ? rest - h * kTileTokens : 0;
+    m.ks[h] = c < valid ? 0xffu : 0u;
     m.vs[h] = 0;
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-      const bool in = 4 * g + e < valid[h];
+      const bool in = 4 * g + e < valid;
       m.bias[h][e] = in ? 0.f : kNegInf;
       m.vs[h] |= in ? 0xffu << (8 * e) : 0u;
     }
@@ -279,6 +296,31 @@ __device__ __forceinline__ uint32_t select_bits(uint32_t mask, uint32_t x, uint3
 template <bool kWide>
 __device__ __forceinline__ void fold_unit(const Unit& u, const Mask& mask, const Query<kWide>& q,
                                           float scale, int c, State<kWide>& st) {
+  constexpr uint32_t kLow16 = 0x05040100u, kHigh16 = 0x07060302u;
+  // Scale bytes to exponent fields; the bits around them do not count.
+  float vs[8];
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    const uint32_t w = select_bits(mask.vs[h], u.vs[h], 0x7f7f7f7fu);
+    vs[4 * h + 0] = __uint_as_float(w << 23);
+    vs[4 * h + 1] = __uint_as_float(w << 15);
+    vs[4 * h + 2] = __uint_as_float(w << 7);
+    vs[4 * h + 3] = __uint_as_float(w >> 1);
+  }
+  const uint32_t code[8] = {u.v[0].x, u.v[0].y, u.v[0].z, u.v[0].w,
+                            u.v[1].x, u.v[1].y, u.v[1].z, u.v[1].w};
+  const auto pairs = [&](auto byte, u32x4& even, u32x4& odd) {
+    uint32_t d[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+      d[e] = __builtin_bit_cast(
+          uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(code[e], vs[e], decltype(byte)::value));
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      even[e] = __builtin_amdgcn_perm(d[2 * e + 1], d[2 * e], kLow16);
+      odd[e] = __builtin_amdgcn_perm(d[2 * e + 1], d[2 * e], kHigh16);
+    }
+  };
   float s[8];
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
@@ -320,7 +362,6 @@ __device__ __forceinline__ void fold_unit(const Unit& u, const Mask& mask, const
       p[0][e] = __float_as_uint(w - __uint_as_float(bits & low));
     }
   }
-  constexpr uint32_t kLow16 = 0x05040100u, kHigh16 = 0x07060302u;
   bf16x8_t pb[kWide ? 2 : 1];
 #pragma unroll
   for (int i = 0; i < (kWide ? 2 : 1); ++i) {
@@ -330,30 +371,6 @@ __device__ __forceinline__ void fold_unit(const Unit& u, const Mask& mask, const
       w[e] = __builtin_amdgcn_perm(p[i][2 * e + 1], p[i][2 * e], kHigh16);
     pb[i] = __builtin_bit_cast(bf16x8_t, w);
   }
-  // Scale bytes to exponent fields; the bits around them do not count.
-  float vs[8];
-#pragma unroll
-  for (int h = 0; h < 2; ++h) {
-    const uint32_t w = select_bits(mask.vs[h], u.vs[h], 0x7f7f7f7fu);
-    vs[4 * h + 0] = __uint_as_float(w << 23);
-    vs[4 * h + 1] = __uint_as_float(w << 15);
-    vs[4 * h + 2] = __uint_as_float(w << 7);
-    vs[4 * h + 3] = __uint_as_float(w >> 1);
-  }
-  const uint32_t code[8] = {u.v[0].x, u.v[0].y, u.v[0].z, u.v[0].w,
-                            u.v[1].x, u.v[1].y, u.v[1].z, u.v[1].w};
-  const auto pairs = [&](auto byte, u32x4& even, u32x4& odd) {
-    uint32_t d[8];
-#pragma unroll
-    for (int e = 0; e < 8; ++e)
-      d[e] = __builtin_bit_cast(
-          uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(code[e], vs[e], decltype(byte)::value));
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      even[e] = __builtin_amdgcn_perm(d[2 * e + 1], d[2 * e], kLow16);
-      odd[e] = __builtin_amdgcn_perm(d[2 * e + 1], d[2 * e], kHigh16);
-    }
-  };
   const auto two_dims = [&](auto byte) {
     constexpr int j = 2 * decltype(byte)::value;
     u32x4 even, odd;
@@ -414,16 +431,16 @@ __device__ __forceinline__ void next_segment(const DecodeArgs& a, Walk& w) {
   w.units = units_of(w.len);
 }
 
-__device__ __forceinline__ const_ints table_of(const DecodeArgs& a, int b) {
-  return (const_ints)(a.block_table + (size_t)b * a.max_blocks);
-}
-
 // Where the walk's unit lies; then on to the next one. At the end of the run the
 // last place stays (its loads are not used).
-__device__ __forceinline__ void next_unit(const DecodeArgs& a, Walk& w, Spot& s) {
+__device__ __forceinline__ void next_unit(const DecodeArgs& a, Walk& w, Segment& seg, Spot& s) {
   if (w.left == 0) return;
-  s = find_unit(a, table_of(a, w.b), w.hc / a.chunks, w.len, w.u);
-  if (--w.left > 0 && (w.u += w.step) >= w.units) next_segment(a, w);
+  s = find_unit(a, seg, w.u);
+  w.u += w.step;
+  if (--w.left > 0 && w.u >= w.units) {
+    next_segment(a, w);
+    seg = segment_of(a, w.b, w.hc, w.len);
+  }
 }
 
 // Sums over the lanes up to this one (of values whose total fits 32 bits): within
@@ -460,7 +477,9 @@ __global__ __launch_bounds__(kThreads, 2) void kv_decode_kernel(DecodeArgs a) {
   // the next unit to fold, `next` is the place of the one after it; neither walk
   // stops at a segment's end.
   Walk at{};
+  Segment seg{};
   Spot next{};
+  const Lanes lanes{16u * lane, (uint32_t)lane, (uint32_t)(16 * g + 4 * (c >> 2))};
   Unit x0, x1;
   RawQuery raw;
   int h0 = 0, nh = 0;  // the q-heads of the segment that raw holds
@@ -475,15 +494,13 @@ __global__ __launch_bounds__(kThreads, 2) void kv_decode_kernel(DecodeArgs a) {
     nh = heads_of(a, at.hc, h0);
     raw = load_query<kWide>(a, at.b, h0, nh, c, g);
     if (wave < units_of(a.capacity)) {
-      next = find_unit(a, table_of(a, at.b), at.hc / a.chunks, a.capacity, wave);
-      load_unit(a, next, lane, x0);
+      next = find_unit(a, segment_of(a, at.b, at.hc, a.capacity), wave);
+      load_unit(a, next, lanes, x0);
     }
     at.len = length_of(a, at.b);
     at.units = units_of(at.len);
     at.left = wave < at.units ? (uint32_t)(at.units - wave + kWaves - 1) / kWaves : 0;
-#pragma unroll
-    for (int h = 0; h < 2; ++h)
-      x0.valid[h] = min(x0.valid[h], max(at.len - wave * kUnit - h * kTileTokens, 0));
+    x0.rest = at.len - wave * kUnit;
   } else {
     // Prefix sums of the requests' units, a slice of them to each lane of one
     // wave (every wave for itself), or to each thread of the workgroup.
@@ -565,14 +582,15 @@ __global__ __launch_bounds__(kThreads, 2) void kv_decode_kernel(DecodeArgs a) {
   const uint32_t slot_floats = (uint32_t)a.heads * kPitch;
   if (at.left > 0) {
     Walk ahead = at;
-    next_unit(a, ahead, next);
+    seg = segment_of(a, at.b, at.hc, at.len);
+    next_unit(a, ahead, seg, next);
     if (a.mode != kPerSegment) {
       // (The queries first: their conversion waits for no tile.)
       nh = heads_of(a, at.hc, h0);
       raw = load_query<kWide>(a, at.b, h0, nh, c, g);
-      load_unit(a, next, lane, x0);
+      load_unit(a, next, lanes, x0);
     }
-    next_unit(a, ahead, next);
+    next_unit(a, ahead, seg, next);
     Mask mask;
     bool unmasked = false;
     while (true) {
@@ -583,7 +601,7 @@ __global__ __launch_bounds__(kThreads, 2) void kv_decode_kernel(DecodeArgs a) {
         starts = wave == 0;
         ends = wave == min(at.units, kWaves) - 1;
       }
-      const int seg = at.b * Hc + at.hc, heads = nh;
+      const int number = at.b * Hc + at.hc, heads = nh;
       uint16_t* const out = a.out + ((size_t)at.b * a.Hq + h0) * kDim;
       const Query<kWide> q = split_query<kWide>(raw, a.flip, c);
       at.left -= (uint32_t)k;
@@ -599,11 +617,11 @@ __global__ __launch_bounds__(kThreads, 2) void kv_decode_kernel(DecodeArgs a) {
       for (int j = 0; j < 8; ++j) st.o[j] = f32x4_t{0.f, 0.f, 0.f, 0.f};
       // Unit x is folded while the loads of the one after it are in flight.
       const auto step = [&](const Unit& x, Unit& y) {
-        load_unit(a, next, lane, y);
-        next_unit(a, ahead, next);
-        const bool whole = x.valid[0] + x.valid[1] == kUnit;
+        load_unit(a, next, lanes, y);
+        next_unit(a, ahead, seg, next);
+        const bool whole = x.rest >= kUnit && x.ok == 3;
         if (!whole || !unmasked) {
-          set_mask(mask, x.valid, c, g);
+          set_mask(mask, x.rest, x.ok, c, g);
           unmasked = whole;
         }
         fold_unit<kWide>(x, mask, q, a.scale, c, st);
@@ -640,10 +658,10 @@ __global__ __launch_bounds__(kThreads, 2) void kv_decode_kernel(DecodeArgs a) {
         const int which = starts ? 1 : 0;
         if (which == 0) {
           flags |= kHasA | (ends ? kEndsA : 0);
-          seg_a = seg;
+          seg_a = number;
         } else {
           flags |= kHasZ;
-          seg_z = seg;
+          seg_z = number;
         }
         if (c < heads) {
           float* dst = slots + (wave * 2 + which) * slot_floats + c * kPitch;
@@ -837,6 +855,7 @@ bool shape_of(int B, int Hq, int Hkv, int num_blocks, int block_size, int max_bl
   if (cap > INT32_MAX - kUnit || B * ((cap + kUnit - 1) / kUnit) > INT32_MAX / (Hkv * s.chunks))
     return false;
   if ((int64_t)B * Hq > (int64_t(1) << 28)) return false;
+  if ((int64_t)block_size / kTileTokens * kTileBytes * Hkv > INT32_MAX) return false;
   s.heads = std::min(s.G, 16);
   s.capacity = (int)cap;
   s.workgroups = num_workgroups;
@@ -905,6 +924,8 @@ extern "C" int kv_decode_mxfp4_launch(const uint16_t* q, const uint8_t* mxfp4_ca
   a.tiles_per_block = block_size / kTileTokens;
   a.max_blocks = max_blocks;
   a.capacity = s.capacity;
+  a.head_bytes = (uint32_t)a.tiles_per_block * kTileBytes;
+  a.block_bytes = a.head_bytes * (uint32_t)Hkv;
   a.tile_div = make_fastdiv((uint32_t)a.tiles_per_block);
   a.head_div = make_fastdiv((uint32_t)(Hkv * s.chunks));
   // (A scale of 0 weighs all tokens alike; the smallest normal does as well and
