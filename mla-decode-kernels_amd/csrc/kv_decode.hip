@@ -48,7 +48,9 @@ using gqa::kNegInf;
 using gqa::wave_max;
 using gqa::wave_sum;
 using gqa::xor16_max;
+using gqa::xor16_sum;
 using gqa::xor32_max;
+using gqa::xor32_sum;
 
 typedef __bf16 bf16x8_t __attribute__((ext_vector_type(8)));
 typedef float f32x4_t __attribute__((ext_vector_type(4)));
@@ -59,13 +61,17 @@ typedef int i32x8_t __attribute__((ext_vector_type(8)));
 constexpr int kUnit = 32;       // tokens a wave takes at a time
 constexpr int kWaves = 8;       // waves of a workgroup
 constexpr int kThreads = 64 * kWaves;
+static_assert((kWaves & (kWaves - 1)) == 0, "heads are dealt out by masks");
 constexpr int kPitch = 132;     // floats of a head's state: acc [128], m, l, pad
 constexpr int kMinUnits = 2;    // units a wave gets before another workgroup joins in
 
 constexpr int kHasA = 1, kEndsA = 2, kHasZ = 4;  // pieces of a share (Record::flags)
 
+// A wave's or a workgroup's cut pieces: what they are, their first row of out
+// (request and q-head) and the number of its rows. (Rows and not segments: whoever
+// folds them has nothing to divide.)
 struct Record {
-  int flags, seg_a, seg_z, pad;
+  int flags, row_a, row_z, heads;  // heads: of A, and of Z from bit 8 on
 };
 
 // How the units are shared out.
@@ -83,11 +89,13 @@ struct DecodeArgs {
   uint16_t* out;
   float* states;     // [workgroups][2][heads][kPitch]
   Record* records;   // [workgroups]
-  int B, Hq, Hkv, G, chunks, heads;  // heads: the largest number of q-heads of a segment
+  int B, Hq, Hkv, G, chunks;
+  int heads;  // the most q-heads of a segment
   int num_blocks, tiles_per_block, max_blocks, capacity;
   uint32_t head_bytes, block_bytes;  // of one head's tiles in a block, of all heads'
   FastDiv tile_div;  // by tiles_per_block
   FastDiv head_div;  // by Hkv * chunks
+  FastDiv chunk_div;  // by chunks
   float scale;       // |scale| log2(e)
   uint32_t flip;     // 0x80008000 for a negative scale: the queries change sign
   int mode;
@@ -220,7 +228,7 @@ struct Segment {
 
 __device__ __forceinline__ Segment segment_of(const DecodeArgs& a, int b, int hc, int len) {
   return Segment{(const_ints)(a.block_table + (size_t)b * a.max_blocks),
-                 (uint32_t)(hc / a.chunks) * a.head_bytes, len};
+                 fastdiv((uint32_t)hc, a.chunk_div) * a.head_bytes, len};
 }
 
 __device__ __forceinline__ Spot find_unit(const DecodeArgs& a, const Segment& seg, int u) {
@@ -400,13 +408,10 @@ __device__ __forceinline__ float inverse(float l) { return l == 0.f ? 0.f : 1.f 
 
 // The q-heads of segment (b, hc): h0 .. h0 + the result - 1.
 __device__ __forceinline__ int heads_of(const DecodeArgs& a, int hc, int& h0) {
-  const int kv_head = hc / a.chunks, first = (hc - kv_head * a.chunks) * 16;
+  const int kv_head = (int)fastdiv((uint32_t)hc, a.chunk_div);
+  const int first = (hc - kv_head * a.chunks) * 16;
   h0 = kv_head * a.G + first;
   return min(16, a.G - first);
-}
-__device__ __forceinline__ int segment_heads(const DecodeArgs& a, int seg, int& b, int& h0) {
-  b = (int)fastdiv((uint32_t)seg, a.head_div);
-  return heads_of(a, seg - b * a.Hkv * a.chunks, h0);
 }
 
 __device__ __forceinline__ int length_of(const DecodeArgs& a, int b) {
@@ -533,9 +538,22 @@ __global__ __launch_bounds__(kThreads, 2) void kv_decode_kernel(DecodeArgs a) {
     const uint32_t want = max(1u, (all + kWaves * kMinUnits - 1) / (kWaves * kMinUnits));
     const uint32_t used = min(want, (uint32_t)nwg);
     const uint32_t each = all / used, more = all - each * used;
-    // Unit p of the line as a place; the request is the one whose prefix sum holds
-    // unit p / Hc of a single head.
-    const auto locate = [&](uint32_t p, Walk& w) {
+    uint32_t w0 = (uint32_t)wg * each + min((uint32_t)wg, more);
+    uint32_t w1 = (uint32_t)wg < used ? w0 + each + ((uint32_t)wg < more ? 1 : 0) : w0;
+    at.step = 1;
+    // The places of the workgroup's ends (kWhole: to move them), then of this
+    // wave's start. (A segment that holds a whole share leaves it empty.)
+    for (int i = a.mode == kWhole && w0 < w1 ? 0 : 2; i < 3; ++i) {
+      uint32_t p = i == 0 ? w0 : w1;
+      if (i == 1 && w1 == all) continue;
+      if (i == 2) {
+        const uint32_t share = w1 - w0;
+        p = w0 + (uint32_t)((uint64_t)share * wave / kWaves);
+        at.left = w0 + (uint32_t)((uint64_t)share * (wave + 1) / kWaves) - p;
+        if (at.left == 0) break;
+      }
+      // Unit p of the line; the request is the one whose prefix sum holds unit
+      // p / Hc of a single head.
       const uint32_t x = fastdiv(p, a.head_div);
       int found = 0;
       uint32_t pre;
@@ -545,40 +563,28 @@ __global__ __launch_bounds__(kThreads, 2) void kv_decode_kernel(DecodeArgs a) {
         pre = (uint32_t)__builtin_amdgcn_readlane((int)before, found - 1);
       } else {
 #pragma unroll
-        for (int i = 0; i < kWaves; ++i)
-          found += __popcll(__builtin_amdgcn_ballot_w64(prefix[i * 64 + lane] <= x));
+        for (int j = 0; j < kWaves; ++j)
+          found += __popcll(__builtin_amdgcn_ballot_w64(prefix[j * 64 + lane] <= x));
         pre = (uint32_t)__builtin_amdgcn_readfirstlane((int)prefix[found - 1]);
       }
-      w.b = __builtin_amdgcn_readfirstlane((found - 1) * slice);
-      w.len = length_of(a, w.b);
-      w.units = units_of(w.len);
-      while (x - pre >= (uint32_t)w.units) {
-        pre += (uint32_t)w.units;
-        w.len = length_of(a, ++w.b);
-        w.units = units_of(w.len);
+      at.b = __builtin_amdgcn_readfirstlane((found - 1) * slice);
+      at.len = length_of(a, at.b);
+      at.units = units_of(at.len);
+      while (x - pre >= (uint32_t)at.units) {
+        pre += (uint32_t)at.units;
+        at.len = length_of(a, ++at.b);
+        at.units = units_of(at.len);
       }
       const uint32_t rem = p - pre * (uint32_t)Hc;
-      w.hc = (int)(rem / (uint32_t)w.units);
-      w.u = (int)(rem - (uint32_t)w.hc * (uint32_t)w.units);
-    };
-    at.step = 1;
-    uint32_t w0 = (uint32_t)wg * each + min((uint32_t)wg, more);
-    uint32_t w1 = (uint32_t)wg < used ? w0 + each + ((uint32_t)wg < more ? 1 : 0) : w0;
-    if (a.mode == kWhole && w0 < w1) {
-      locate(w0, at);
-      if (at.u > 0) w0 += (uint32_t)(at.units - at.u);
-      if (w1 < all) {
-        locate(w1, at);
-        if (at.u > 0) w1 += (uint32_t)(at.units - at.u);
-      }
+      at.hc = (int)(rem / (uint32_t)at.units);
+      at.u = (int)(rem - (uint32_t)at.hc * (uint32_t)at.units);
+      const uint32_t up = at.u > 0 ? (uint32_t)(at.units - at.u) : 0;
+      if (i == 0) w0 += up;
+      if (i == 1) w1 += up;
     }
-    const uint32_t share = w1 - w0;  // (a segment that holds a whole share: 0)
-    const uint32_t p0 = w0 + (uint32_t)((uint64_t)share * wave / kWaves);
-    at.left = w0 + (uint32_t)((uint64_t)share * (wave + 1) / kWaves) - p0;
-    if (at.left > 0) locate(p0, at);
   }
 
-  int flags = 0, seg_a = 0, seg_z = 0;
+  Record mine{0, 0, 0, 0};
   const uint32_t slot_floats = (uint32_t)a.heads * kPitch;
   if (at.left > 0) {
     Walk ahead = at;
@@ -601,8 +607,7 @@ __global__ __launch_bounds__(kThreads, 2) void kv_decode_kernel(DecodeArgs a) {
         starts = wave == 0;
         ends = wave == min(at.units, kWaves) - 1;
       }
-      const int number = at.b * Hc + at.hc, heads = nh;
-      uint16_t* const out = a.out + ((size_t)at.b * a.Hq + h0) * kDim;
+      const int row = at.b * a.Hq + h0, heads = nh;
       const Query<kWide> q = split_query<kWide>(raw, a.flip, c);
       at.left -= (uint32_t)k;
       if (at.left > 0) {  // the next segment's queries are on their way meanwhile
@@ -644,7 +649,7 @@ __global__ __launch_bounds__(kThreads, 2) void kv_decode_kernel(DecodeArgs a) {
       const float l = st.l[0];
       if (starts && ends) {
         if (c < heads) {
-          uint16_t* dst = out + c * kDim + 32 * g;
+          uint16_t* dst = a.out + (size_t)(row + c) * kDim + 32 * g;
           const float r = inverse(l);
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
@@ -657,11 +662,13 @@ __global__ __launch_bounds__(kThreads, 2) void kv_decode_kernel(DecodeArgs a) {
       } else {
         const int which = starts ? 1 : 0;
         if (which == 0) {
-          flags |= kHasA | (ends ? kEndsA : 0);
-          seg_a = number;
+          mine.flags |= kHasA | (ends ? kEndsA : 0);
+          mine.row_a = row;
+          mine.heads |= heads;
         } else {
-          flags |= kHasZ;
-          seg_z = number;
+          mine.flags |= kHasZ;
+          mine.row_z = row;
+          mine.heads |= heads << 8;
         }
         if (c < heads) {
           float* dst = slots + (wave * 2 + which) * slot_floats + c * kPitch;
@@ -680,7 +687,7 @@ __global__ __launch_bounds__(kThreads, 2) void kv_decode_kernel(DecodeArgs a) {
       if (at.left == 0) break;
     }
   }
-  if (lane == 0) meta[wave] = Record{flags, seg_a, seg_z, 0};
+  if (lane == 0) meta[wave] = mine;
   __syncthreads();
 
   // The pieces of a segment cut between waves are neighbours: a run starts
@@ -710,19 +717,17 @@ __global__ __launch_bounds__(kThreads, 2) void kv_decode_kernel(DecodeArgs a) {
     const bool ends = last != 0;
     const uint32_t upto = ends ? (last & -last) * 2 - 1 : ~0u;
     const uint32_t as = has_a & behind & upto;  // waves whose A pieces belong to it
-    const int seg = __builtin_amdgcn_readlane(which ? m.seg_z : m.seg_a, w);
+    const int row = __builtin_amdgcn_readlane(which ? m.row_z : m.row_a, w);
+    const int nh = __builtin_amdgcn_readlane(which ? m.heads >> 8 : m.heads & 255, w);
     const bool to_out = which && ends;
     if (!which) {
       rec.flags |= kHasA | (ends ? kEndsA : 0);
-      rec.seg_a = seg;
+      rec.row_a = row;
+      rec.heads = nh;
     } else if (!ends) {
       rec.flags |= kHasZ;
-      rec.seg_z = seg;
     }
-    int sb, h0;
-    const int nh = segment_heads(a, seg, sb, h0);
-    int h = wave - turn % kWaves;
-    if (h < 0) h += kWaves;
+    int h = (wave - turn) & (kWaves - 1);
     turn += nh;
     for (; h < nh; h += kWaves) {
       // Piece i: wave i's A, or piece kWaves: the Z that starts the run. A lane
@@ -731,12 +736,12 @@ __global__ __launch_bounds__(kThreads, 2) void kv_decode_kernel(DecodeArgs a) {
       const auto piece = [&](int i) {
         return slots + (uint32_t)(i == kWaves ? w * 2 + 1 : i * 2) * slot_floats + h * kPitch;
       };
-      const int mine = min(lane, kWaves);
-      const float2 ml = *reinterpret_cast<const float2*>(piece(mine) + kDim);
+      const int own = min(lane, kWaves);
+      const float2 ml = *reinterpret_cast<const float2*>(piece(own) + kDim);
       float2 v[kWaves + 1];
 #pragma unroll
       for (int i = 0; i <= kWaves; ++i) v[i] = reinterpret_cast<const float2*>(piece(i))[lane];
-      const bool counts = lane <= kWaves && (live >> mine & 1);
+      const bool counts = lane <= kWaves && (live >> own & 1);
       const float M = wave_max(counts ? ml.x : kNegInf);
       const float fl = counts && M != kNegInf ? exp2_fast(ml.x - M) : 0.f;
       float L = counts ? ml.y * fl : 0.f, x = 0.f, y = 0.f;
@@ -750,7 +755,7 @@ __global__ __launch_bounds__(kThreads, 2) void kv_decode_kernel(DecodeArgs a) {
         y = fmaf(in ? v[i].y : 0.f, f, y);
       }
       if (to_out) {
-        reinterpret_cast<uint32_t*>(a.out + ((size_t)sb * a.Hq + h0 + h) * kDim)[lane] =
+        reinterpret_cast<uint32_t*>(a.out + (size_t)(row + h) * kDim)[lane] =
             pack2(x * inverse(L), y * inverse(L));
       } else {
         float* dst = a.states + ((size_t)wg * 2 + which) * slot_floats + h * kPitch;
@@ -773,67 +778,111 @@ __global__ __launch_bounds__(kThreads, 2) void kv_decode_kernel(DecodeArgs a) {
 }
 
 // Segments cut between workgroups: the workgroup whose first piece ends one
-// folds it, from the one whose last piece starts it. A wave to each head; pieces in
-// share order.
-constexpr int kMergeWaves = 4;
-__global__ __launch_bounds__(64 * kMergeWaves) void kv_decode_merge_kernel(DecodeArgs a) {
+// folds it, from the one whose last piece starts it. 16 waves share the heads,
+// and what is left of them a head's pieces, whose parts meet in LDS. A row of 16
+// lanes takes a piece, 8 dims a lane, kBatch pieces in flight: the kernel is one
+// chain of latencies (records, states, a sum over the rows), and every step
+// that a wave does not take alone shortens it. One request of 32768 tokens (32
+// pieces to a segment): SINGLE us in all where each wave takes a head's pieces
+// one after the other, two dims a lane, NOW us so.
+struct MergeArgs {
+  const Record* records;
+  const float* states;
+  uint16_t* out;
+  uint32_t slot_floats;
+  int head_bits;  // waves for 2^head_bits heads
+};
+constexpr int kMergeWaves = 16;
+constexpr int kBatch = 4;
+__global__ __launch_bounds__(64 * kMergeWaves) void kv_decode_merge_kernel(MergeArgs a) {
+  __shared__ float row[kMergeWaves][kDim];
+  __shared__ float2 weight[kMergeWaves];
   const int wg = blockIdx.x, lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   // Lane i reads record wg - i: the workgroup's own, and those in front.
-  Record r = a.records[max(wg - lane, 0)];
+  const Record r = a.records[max(wg - lane, 0)];
   const int flags = __builtin_amdgcn_readfirstlane(r.flags);
-  const int seg = __builtin_amdgcn_readfirstlane(r.seg_a);
+  const int first_row = __builtin_amdgcn_readfirstlane(r.row_a);
+  const int nh = __builtin_amdgcn_readfirstlane(r.heads);
   if ((flags & (kHasA | kEndsA)) != (kHasA | kEndsA)) return;
-  int from = -1;
   uint64_t hit = __builtin_amdgcn_ballot_w64(lane > 0 && lane <= wg && (r.flags & kHasZ) != 0);
-  for (int base = wg;; hit = __builtin_amdgcn_ballot_w64(
-                           lane <= base && (a.records[max(base - lane, 0)].flags & kHasZ) != 0)) {
-    if (hit) {
-      from = base - (int)__builtin_ctzll(hit);
-      break;
-    }
+  int base = wg;
+  while (!hit) {
     base -= 64;
     if (base < 0) return;
+    hit = __builtin_amdgcn_ballot_w64(lane <= base &&
+                                      (a.records[max(base - lane, 0)].flags & kHasZ) != 0);
   }
-  int b, h0;
-  const int nh = segment_heads(a, seg, b, h0);
-  const int h = (int)blockIdx.y * kMergeWaves + (threadIdx.x >> 6);
-  if (h >= nh) return;
-  const uint32_t slot_floats = (uint32_t)a.heads * kPitch;
-  // (Shares go to the first workgroups, so all from `from` to wg have a piece.)
-  const float* const states = a.states + (size_t)from * 2 * slot_floats + h * kPitch;
-  const auto state = [&](int i) {  // piece i: a Z piece, then A pieces
-    return states + (size_t)(i ? 2 * (uint32_t)i : 1u) * slot_floats;
-  };
-  const int n = wg - from + 1;
-  // 32 pieces at a time: their rows and, a piece to a lane, their m and l go out
-  // together with the loads of all maxima, so that up to 32 pieces take one
-  // round trip.
-  constexpr int kBatch = 32;
-  float mloc = kNegInf, M = kNegInf;
-  for (int i = lane; i < n; i += 64) mloc = fmaxf(mloc, state(i)[kDim]);
-  float L = 0.f, x = 0.f, y = 0.f;
-  for (int i0 = 0; i0 < n; i0 += kBatch) {
-    float2 v[kBatch];
+  const int from = base - (int)__builtin_ctzll(hit);
+  const int parts = kMergeWaves >> a.head_bits;
+  const int h = wave & ((1 << a.head_bits) - 1), part = wave >> a.head_bits;
+  const uint32_t slot_floats = a.slot_floats;
+  // (Shares go to the first workgroups, so all from `from` to wg have a piece: a Z,
+  // then As.)
+  const float* const states =
+      a.states + (size_t)from * 2 * slot_floats + (h < nh ? h : 0) * kPitch;
+  const int n = wg - from + 1, i = lane & 15;
+  float M = kNegInf, L = 0.f, x[8] = {};
+  for (int p0 = part * 4 + (lane >> 4); p0 - (lane >> 4) < n; p0 += 4 * kBatch * parts) {
+    float2 ml[kBatch];
+    f32x4_t v[kBatch][2];
 #pragma unroll
-    for (int i = 0; i < kBatch; ++i)
-      v[i] = reinterpret_cast<const float2*>(state(min(i0 + i, n - 1)))[lane];
-    const float2 ml =
-        *reinterpret_cast<const float2*>(state(min(i0 + (lane & (kBatch - 1)), n - 1)) + kDim);
-    if (i0 == 0) M = wave_max(mloc);
-    const float fl = M == kNegInf ? 0.f : exp2_fast(ml.x - M);
+    for (int k = 0; k < kBatch; ++k) {
+      const int p = p0 + 4 * k * parts;
+      const float* s = states + (size_t)(p == 0 ? 1u : 2 * (uint32_t)min(p, n - 1)) * slot_floats;
+      ml[k] = *reinterpret_cast<const float2*>(s + kDim);
+      if (p >= n) ml[k].x = kNegInf;
 #pragma unroll
-    for (int i = 0; i < kBatch; ++i) {
-      const float f = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(fl), i));
-      const float l = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(ml.y), i));
-      if (i0 + i < n) {
-        L = fmaf(l, f, L);
-        x = fmaf(v[i].x, f, x);
-        y = fmaf(v[i].y, f, y);
-      }
+      for (int e = 0; e < 2; ++e) v[k][e] = reinterpret_cast<const f32x4_t*>(s + 8 * i)[e];
+    }
+    float m = ml[0].x;
+#pragma unroll
+    for (int k = 1; k < kBatch; ++k) m = fmaxf(m, ml[k].x);
+    m = fmaxf(M, xor32_max(xor16_max(m)));
+    const float old = m == kNegInf ? 1.f : exp2_fast(M - m);
+    M = m;
+    L *= old;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) x[e] *= old;
+#pragma unroll
+    for (int k = 0; k < kBatch; ++k) {
+      if (p0 + 4 * k * parts >= n) continue;
+      const float f = m == kNegInf ? 0.f : exp2_fast(ml[k].x - m);
+      L = fmaf(ml[k].y, f, L);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) x[e] = fmaf(v[k][e >> 2][e & 3], f, x[e]);
     }
   }
-  reinterpret_cast<uint32_t*>(a.out + ((size_t)b * a.Hq + h0 + h) * kDim)[lane] =
-      pack2(x * inverse(L), y * inverse(L));
+  L = xor32_sum(xor16_sum(L));
+#pragma unroll
+  for (int e = 0; e < 8; ++e) x[e] = xor32_sum(xor16_sum(x[e]));
+  uint16_t* const out = a.out + (size_t)(first_row + h) * kDim;
+  if (parts == 1) {
+    if (h >= nh || lane >= 16) return;
+    const float r = inverse(L);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) x[e] *= r;
+    reinterpret_cast<uint4*>(out)[i] = pack8(x);
+    return;
+  }
+  if (lane < 16) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) row[wave][8 * i + e] = x[e];
+    if (lane == 0) weight[wave] = make_float2(M, L);
+  }
+  __syncthreads();
+  if (part > 0 || h >= nh) return;
+  float top = kNegInf, sum = 0.f, x0 = 0.f, x1 = 0.f;
+  for (int p = h; p < kMergeWaves; p += 1 << a.head_bits) top = fmaxf(top, weight[p].x);
+  for (int p = h; p < kMergeWaves; p += 1 << a.head_bits) {
+    const float2 w = weight[p];
+    const float f = top == kNegInf ? 0.f : exp2_fast(w.x - top);
+    sum = fmaf(w.y, f, sum);
+    x0 = fmaf(row[p][2 * lane], f, x0);
+    x1 = fmaf(row[p][2 * lane + 1], f, x1);
+  }
+  const float r1 = inverse(sum);
+  reinterpret_cast<uint32_t*>(out)[lane] = pack2(x0 * r1, x1 * r1);
 }
 
 struct Shape {
@@ -928,6 +977,7 @@ extern "C" int kv_decode_mxfp4_launch(const uint16_t* q, const uint8_t* mxfp4_ca
   a.block_bytes = a.head_bytes * (uint32_t)Hkv;
   a.tile_div = make_fastdiv((uint32_t)a.tiles_per_block);
   a.head_div = make_fastdiv((uint32_t)(Hkv * s.chunks));
+  a.chunk_div = make_fastdiv((uint32_t)s.chunks);
   // (A scale of 0 weighs all tokens alike; the smallest normal does as well and
   // keeps 0 * infinity out of the kernel.)
   a.scale = std::max(fabsf(scale) * gqa::kLog2e, 1.17549435e-38f);
@@ -943,7 +993,8 @@ extern "C" int kv_decode_mxfp4_launch(const uint16_t* q, const uint8_t* mxfp4_ca
   kernel<<<s.workgroups, kThreads, lds, stream>>>(a);
   hipError_t e = hipGetLastError();
   if (e != hipSuccess || s.mode != kBalanced) return e;
-  kv_decode_merge_kernel<<<dim3(s.workgroups, (s.heads + kMergeWaves - 1) / kMergeWaves),
-                           64 * kMergeWaves, 0, stream>>>(a);
+  MergeArgs m{a.records, a.states, out, (uint32_t)s.heads * kPitch, 0};
+  while (1 << m.head_bits < s.heads) ++m.head_bits;
+  kv_decode_merge_kernel<<<s.workgroups, 64 * kMergeWaves, 0, stream>>>(m);
   return hipGetLastError();
 }
