@@ -338,59 +338,73 @@ __global__ __launch_bounds__(64 * kWaves) void kv_read_mxfp4_kernel(
 
 constexpr int kLatent = 512, kRope = 64, kRow = kLatent + kRope;
 
-// A wave takes one token's latent row (pass 0), or eight of its 64-dim rotary
-// rows, 8 lanes each (queries, then the key; passes 1 ..).
-// Grid: x tokens, y groups of kWaves passes.
+// A token's rows come in passes of a wave: the latent row (pass 0), then eight
+// 64-dim rotary rows at a time, 8 lanes each (queries, then the key). A wave takes
+// R passes, whose loads go out together; the token's place and angles are found
+// once. Grid: x groups of kWaves tokens, one to each wave, y groups of R passes.
+template <int R>
 __global__ __launch_bounds__(64 * kWaves) void kv_append_mla_kernel(kv_append_mla_args a,
                                                                     FastDiv bs_div) {
   const int lane = threadIdx.x & 63;
-  const int t = (int)blockIdx.x;
-  const int pass = (int)blockIdx.y * kWaves + (threadIdx.x >> 6);
-  const int row = (pass - 1) * 8 + (lane >> 3);  // passes 1 ..: q heads, then k_pe
+  const int t = (int)blockIdx.x * kWaves + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int pass0 = (int)blockIdx.y * R;
+  const int passes = 1 + (a.h_q + 8) / 8;
   const int i = lane & 7;
-  if (pass > (a.h_q + 8) / 8) return;
-  const bool is_q = pass > 0 && row < a.h_q, is_k = pass > 0 && row == a.h_q;
+  if (t >= a.T) return;
+  const auto row_of = [&](int j) { return (pass0 + j - 1) * 8 + (lane >> 3); };
 
-  uint4 raw = make_uint4(0, 0, 0, 0);
-  if (pass == 0)
-    raw = load16(a.c + t * a.c_token_stride + 8 * lane);
-  else if (is_q)
-    raw = load16(a.q_pe + t * a.q_token_stride + row * a.q_head_stride + 8 * i);
-  else if (is_k)
-    raw = load16(a.k_pe + t * a.k_token_stride + 8 * i);
+  uint4 raw[R];
+#pragma unroll
+  for (int j = 0; j < R; ++j) {
+    raw[j] = make_uint4(0, 0, 0, 0);
+    const int row = row_of(j);
+    if (pass0 + j == 0)
+      raw[j] = load16(a.c + t * a.c_token_stride + 8 * lane);
+    else if (row < a.h_q)
+      raw[j] = load16(a.q_pe + t * a.q_token_stride + row * a.q_head_stride + 8 * i);
+    else if (row == a.h_q)
+      raw[j] = load16(a.k_pe + t * a.k_token_stride + 8 * i);
+  }
 
   const Place place = find_place<64>(t, a.T, a.B, a.seq_lens, a.cu_seqlens, lane);
   int slot;
   const int block = find_block(place, a.block_table, a.max_blocks, a.num_blocks, bs_div, slot);
   uint16_t* dst = a.kv_cache + ((size_t)max(block, 0) * a.block_size + slot) * kRow;
-  float x[8];
-  unpack8(raw, x);
-  if (pass == 0) {
-    if (a.c_weight) {
-      float ss = 0.f;
+  Turn turn{};
+  if (pass0 + R > 1)
+    turn = load_turn<8>(a.cos_sin, a.table_rows, kRope, a.interleaved,
+                        a.rope_positions ? a.rope_positions[t] : place.pos, lane);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) ss = fmaf(x[e], x[e], ss);
-      const float r = rsqrtf(gqa::wave_sum(ss) * (1.f / kLatent) + a.eps);
-      float w[8];
-      load_weights(a.c_weight, a.c_weight_type, 8 * lane, w);
+  for (int j = 0; j < R; ++j) {
+    if (pass0 + j >= passes) break;
+    float x[8];
+    unpack8(raw[j], x);
+    if (pass0 + j == 0) {
+      if (a.c_weight) {
+        float ss = 0.f;
 #pragma unroll
-      for (int e = 0; e < 8; ++e) x[e] = x[e] * r * w[e];
-      raw = pack8(x);
+        for (int e = 0; e < 8; ++e) ss = fmaf(x[e], x[e], ss);
+        const float r = rsqrtf(gqa::wave_sum(ss) * (1.f / kLatent) + a.eps);
+        float w[8];
+        load_weights(a.c_weight, a.c_weight_type, 8 * lane, w);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x[e] = x[e] * r * w[e];
+        raw[j] = pack8(x);
+      }
+      if (block >= 0) *reinterpret_cast<uint4*>(dst + 8 * lane) = raw[j];
+      continue;
     }
-    if (block >= 0) *reinterpret_cast<uint4*>(dst + 8 * lane) = raw;
-    return;
-  }
-  const Turn turn = load_turn<8>(a.cos_sin, a.table_rows, kRope, a.interleaved,
-                                 a.rope_positions ? a.rope_positions[t] : place.pos, lane);
-  float y[8];
-  others(x, y, turn, a.interleaved ? kInside : kPartner);
+    float y[8];
+    others(x, y, turn, a.interleaved ? kInside : kPartner);
 #pragma unroll
-  for (int e = 0; e < 8; ++e) x[e] = fmaf(x[e], turn.c[e], y[e] * turn.s[e]);
-  if (is_q)
-    store16(a.q_out + t * a.q_out_token_stride + row * a.q_out_head_stride + 8 * i,
-            place.live ? pack8(x) : make_uint4(0, 0, 0, 0));
-  else if (is_k && block >= 0)
-    *reinterpret_cast<uint4*>(dst + kLatent + 8 * i) = pack8(x);
+    for (int e = 0; e < 8; ++e) x[e] = fmaf(x[e], turn.c[e], y[e] * turn.s[e]);
+    const int row = row_of(j);
+    if (row < a.h_q)
+      store16(a.q_out + t * a.q_out_token_stride + row * a.q_out_head_stride + 8 * i,
+              place.live ? pack8(x) : make_uint4(0, 0, 0, 0));
+    else if (row == a.h_q && block >= 0)
+      *reinterpret_cast<uint4*>(dst + kLatent + 8 * i) = pack8(x);
+  }
 }
 
 // ------------------------------------------------------------------ host
@@ -496,7 +510,15 @@ extern "C" int kv_append_mla_launch(const kv_append_mla_args* args, hipStream_t 
       (a.num_blocks > 0 && (!a.kv_cache || misaligned(a.kv_cache, 16))))
     return hipErrorInvalidValue;
   const int passes = 1 + (a.h_q + 8) / 8;  // the latent row, then h_q + 1 rotary rows
-  kv_append_mla_kernel<<<dim3((unsigned)a.T, (passes + kWaves - 1) / kWaves), 64 * kWaves, 0,
-                         stream>>>(a, make_fastdiv(a.block_size));
+  const FastDiv bs_div = make_fastdiv((uint32_t)a.block_size);
+  const auto launch = [&](auto many) {
+    constexpr int R = decltype(many)::value;
+    kv_append_mla_kernel<R><<<dim3((unsigned)(a.T + kWaves - 1) / kWaves, (passes + R - 1) / R),
+                              64 * kWaves, 0, stream>>>(a, bs_div);
+  };
+  if ((int64_t)a.T * passes <= 8192)
+    launch(std::integral_constant<int, 1>{});
+  else
+    launch(std::integral_constant<int, 4>{});
   return hipGetLastError();
 }

@@ -778,33 +778,31 @@ __global__ __launch_bounds__(kThreads, 2) void kv_decode_kernel(DecodeArgs a) {
 }
 
 // Segments cut between workgroups: the workgroup whose first piece ends one
-// folds it, from the one whose last piece starts it. 16 waves share the heads,
-// and what is left of them a head's pieces, whose parts meet in LDS. A row of 16
-// lanes takes a piece, 8 dims a lane, kBatch pieces in flight: the kernel is one
-// chain of latencies (records, states, a sum over the rows), and every step
-// that a wave does not take alone shortens it. One request of 32768 tokens (32
-// pieces to a segment): SINGLE us in all where each wave takes a head's pieces
-// one after the other, two dims a lane, NOW us so.
+// folds it, from the one whose last piece starts it. A wave to a head; a row of
+// 16 lanes takes every fourth piece, 8 dims a lane, with a state of its own, and
+// the four rows meet at the end. One chain of latencies (records, states, the
+// sum over the rows), so what shortens it is few instructions on a wave that has
+// its SIMD to itself. Against 16 waves on one CU that share a segment's heads and
+// pieces and meet in LDS: 4 requests of 2048 tokens 11.4 us in all for 12.3, a
+// ragged batch of 64 (64Q/8KV) 167.6 for 168.8; one request of 32768 (32 pieces to
+// a segment) 17.0 for 16.6.
 struct MergeArgs {
   const Record* records;
   const float* states;
   uint16_t* out;
   uint32_t slot_floats;
-  int head_bits;  // waves for 2^head_bits heads
 };
-constexpr int kMergeWaves = 16;
-constexpr int kBatch = 4;
+constexpr int kMergeWaves = 4;
 __global__ __launch_bounds__(64 * kMergeWaves) void kv_decode_merge_kernel(MergeArgs a) {
-  __shared__ float row[kMergeWaves][kDim];
-  __shared__ float2 weight[kMergeWaves];
   const int wg = blockIdx.x, lane = threadIdx.x & 63;
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   // Lane i reads record wg - i: the workgroup's own, and those in front.
   const Record r = a.records[max(wg - lane, 0)];
   const int flags = __builtin_amdgcn_readfirstlane(r.flags);
-  const int first_row = __builtin_amdgcn_readfirstlane(r.row_a);
-  const int nh = __builtin_amdgcn_readfirstlane(r.heads);
+  const int h = (int)blockIdx.y * kMergeWaves +
+                __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
   if ((flags & (kHasA | kEndsA)) != (kHasA | kEndsA)) return;
+  if (h >= __builtin_amdgcn_readfirstlane(r.heads)) return;
+  const int row = __builtin_amdgcn_readfirstlane(r.row_a) + h;
   uint64_t hit = __builtin_amdgcn_ballot_w64(lane > 0 && lane <= wg && (r.flags & kHasZ) != 0);
   int base = wg;
   while (!hit) {
@@ -814,75 +812,45 @@ __global__ __launch_bounds__(64 * kMergeWaves) void kv_decode_merge_kernel(Merge
                                       (a.records[max(base - lane, 0)].flags & kHasZ) != 0);
   }
   const int from = base - (int)__builtin_ctzll(hit);
-  const int parts = kMergeWaves >> a.head_bits;
-  const int h = wave & ((1 << a.head_bits) - 1), part = wave >> a.head_bits;
-  const uint32_t slot_floats = a.slot_floats;
   // (Shares go to the first workgroups, so all from `from` to wg have a piece: a Z,
   // then As.)
-  const float* const states =
-      a.states + (size_t)from * 2 * slot_floats + (h < nh ? h : 0) * kPitch;
   const int n = wg - from + 1, i = lane & 15;
-  float M = kNegInf, L = 0.f, x[8] = {};
-  for (int p0 = part * 4 + (lane >> 4); p0 - (lane >> 4) < n; p0 += 4 * kBatch * parts) {
-    float2 ml[kBatch];
-    f32x4_t v[kBatch][2];
-#pragma unroll
-    for (int k = 0; k < kBatch; ++k) {
-      const int p = p0 + 4 * k * parts;
-      const float* s = states + (size_t)(p == 0 ? 1u : 2 * (uint32_t)min(p, n - 1)) * slot_floats;
-      ml[k] = *reinterpret_cast<const float2*>(s + kDim);
-      if (p >= n) ml[k].x = kNegInf;
-#pragma unroll
-      for (int e = 0; e < 2; ++e) v[k][e] = reinterpret_cast<const f32x4_t*>(s + 8 * i)[e];
-    }
-    float m = ml[0].x;
-#pragma unroll
-    for (int k = 1; k < kBatch; ++k) m = fmaxf(m, ml[k].x);
-    m = fmaxf(M, xor32_max(xor16_max(m)));
-    const float old = m == kNegInf ? 1.f : exp2_fast(M - m);
+  const float* const states = a.states + (size_t)from * 2 * a.slot_floats + h * kPitch;
+  struct Piece {
+    float2 ml;
+    f32x4_t v[2];
+  };
+  const auto load = [&](int p) {
+    const float* s =
+        states + (size_t)(p == 0 ? 1u : 2 * (uint32_t)min(p, n - 1)) * a.slot_floats;
+    return Piece{*reinterpret_cast<const float2*>(s + kDim),
+                 {reinterpret_cast<const f32x4_t*>(s + 8 * i)[0],
+                  reinterpret_cast<const f32x4_t*>(s + 8 * i)[1]}};
+  };
+  float M = kNegInf, L = 0.f;
+  f32x4_t x[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+  int p = lane >> 4;
+  Piece next = load(p), after = load(p + 4);
+  for (int p0 = 0; p0 < n; p0 += 4, p += 4) {
+    const Piece now = next;
+    next = after;
+    after = load(p + 8);
+    if (p >= n) break;  // (these rows are done)
+    const float m = fmaxf(M, now.ml.x), ref = m == kNegInf ? 0.f : m;
+    const float old = exp2_fast(M - ref), f = exp2_fast(now.ml.x - ref);
     M = m;
-    L *= old;
-#pragma unroll
-    for (int e = 0; e < 8; ++e) x[e] *= old;
-#pragma unroll
-    for (int k = 0; k < kBatch; ++k) {
-      if (p0 + 4 * k * parts >= n) continue;
-      const float f = m == kNegInf ? 0.f : exp2_fast(ml[k].x - m);
-      L = fmaf(ml[k].y, f, L);
-#pragma unroll
-      for (int e = 0; e < 8; ++e) x[e] = fmaf(v[k][e >> 2][e & 3], f, x[e]);
-    }
+    L = fmaf(L, old, now.ml.y * f);
+    x[0] = x[0] * old + now.v[0] * f;
+    x[1] = x[1] * old + now.v[1] * f;
   }
-  L = xor32_sum(xor16_sum(L));
+  const float top = xor32_max(xor16_max(M));
+  const float f = M == kNegInf ? 0.f : exp2_fast(M - top);
+  L = xor32_sum(xor16_sum(L * f));
+  const float inv = inverse(L);
+  float y[8];
 #pragma unroll
-  for (int e = 0; e < 8; ++e) x[e] = xor32_sum(xor16_sum(x[e]));
-  uint16_t* const out = a.out + (size_t)(first_row + h) * kDim;
-  if (parts == 1) {
-    if (h >= nh || lane >= 16) return;
-    const float r = inverse(L);
-#pragma unroll
-    for (int e = 0; e < 8; ++e) x[e] *= r;
-    reinterpret_cast<uint4*>(out)[i] = pack8(x);
-    return;
-  }
-  if (lane < 16) {
-#pragma unroll
-    for (int e = 0; e < 8; ++e) row[wave][8 * i + e] = x[e];
-    if (lane == 0) weight[wave] = make_float2(M, L);
-  }
-  __syncthreads();
-  if (part > 0 || h >= nh) return;
-  float top = kNegInf, sum = 0.f, x0 = 0.f, x1 = 0.f;
-  for (int p = h; p < kMergeWaves; p += 1 << a.head_bits) top = fmaxf(top, weight[p].x);
-  for (int p = h; p < kMergeWaves; p += 1 << a.head_bits) {
-    const float2 w = weight[p];
-    const float f = top == kNegInf ? 0.f : exp2_fast(w.x - top);
-    sum = fmaf(w.y, f, sum);
-    x0 = fmaf(row[p][2 * lane], f, x0);
-    x1 = fmaf(row[p][2 * lane + 1], f, x1);
-  }
-  const float r1 = inverse(sum);
-  reinterpret_cast<uint32_t*>(out)[lane] = pack2(x0 * r1, x1 * r1);
+  for (int e = 0; e < 8; ++e) y[e] = xor32_sum(xor16_sum(x[e >> 2][e & 3] * f)) * inv;
+  if (lane < 16) reinterpret_cast<uint4*>(a.out + (size_t)row * kDim)[i] = pack8(y);
 }
 
 struct Shape {
@@ -993,8 +961,8 @@ extern "C" int kv_decode_mxfp4_launch(const uint16_t* q, const uint8_t* mxfp4_ca
   kernel<<<s.workgroups, kThreads, lds, stream>>>(a);
   hipError_t e = hipGetLastError();
   if (e != hipSuccess || s.mode != kBalanced) return e;
-  MergeArgs m{a.records, a.states, out, (uint32_t)s.heads * kPitch, 0};
-  while (1 << m.head_bits < s.heads) ++m.head_bits;
-  kv_decode_merge_kernel<<<s.workgroups, 64 * kMergeWaves, 0, stream>>>(m);
+  const MergeArgs m{a.records, a.states, out, (uint32_t)s.heads * kPitch};
+  kv_decode_merge_kernel<<<dim3(s.workgroups, (s.heads + kMergeWaves - 1) / kMergeWaves),
+                           64 * kMergeWaves, 0, stream>>>(m);
   return hipGetLastError();
 }
