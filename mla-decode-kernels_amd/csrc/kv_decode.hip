@@ -65,6 +65,8 @@ static_assert((kWaves & (kWaves - 1)) == 0, "heads are dealt out by masks");
 constexpr int kPitch = 132;     // floats of a head's state: acc [128], m, l, pad
 constexpr int kMinUnits = 2;    // units a wave gets before another workgroup joins in
 
+constexpr int kSlice = 4;       // requests a lane keeps the prefix sums of (8 cost 512 requests 0.7 us)
+
 constexpr int kHasA = 1, kEndsA = 2, kHasZ = 4;  // pieces of a share (Record::flags)
 
 // A wave's or a workgroup's cut pieces: what they are, their first row of out
@@ -507,15 +509,27 @@ __global__ __launch_bounds__(kThreads, 2) void kv_decode_kernel(DecodeArgs a) {
     at.left = wave < at.units ? (uint32_t)(at.units - wave + kWaves - 1) / kWaves : 0;
     x0.rest = at.len - wave * kUnit;
   } else {
-    // Prefix sums of the requests' units, a slice of them to each lane of one
-    // wave (every wave for itself), or to each thread of the workgroup.
-    const bool small = a.B <= 64;
-    const int slice = small ? 1 : (a.B + kThreads - 1) / kThreads;
-    const int mine = small ? lane : tid;
-    uint32_t sum = 0;
-    for (int i = 0; i < slice; ++i) {
-      const int r = mine * slice + i;
-      if (r < a.B) sum += (uint32_t)units_of(min(max(a.seq_lens[r], 0), a.capacity));
+    // Prefix sums of the requests' units, a slice of them to each lane: up to
+    // kSlice each, every wave for itself and in registers; beyond that a slice to
+    // each thread of the workgroup, through LDS.
+    const bool small = a.B <= 64 * kSlice;
+    const int slice = small ? (a.B + 63) / 64 : (a.B + kThreads - 1) / kThreads;
+    const int first = (small ? lane : tid) * slice;
+    uint32_t sum = 0, upto[kSlice];  // upto: the lane's units with request first + j
+    if (small) {
+      int lens[kSlice];
+#pragma unroll
+      for (int j = 0; j < kSlice; ++j)
+        if (j < slice) lens[j] = first + j < a.B ? a.seq_lens[first + j] : 0;
+#pragma unroll
+      for (int j = 0; j < kSlice; ++j) {
+        if (j < slice) sum += (uint32_t)units_of(min(max(lens[j], 0), a.capacity));
+        upto[j] = sum;
+      }
+    } else {
+      for (int i = 0; i < slice; ++i)
+        if (first + i < a.B)
+          sum += (uint32_t)units_of(min(max(a.seq_lens[first + i], 0), a.capacity));
     }
     const uint32_t inc = wave_prefix(sum);
     uint32_t base = 0, total = (uint32_t)__builtin_amdgcn_readlane((int)inc, 63);
@@ -555,25 +569,35 @@ __global__ __launch_bounds__(kThreads, 2) void kv_decode_kernel(DecodeArgs a) {
       // Unit p of the line; the request is the one whose prefix sum holds unit
       // p / Hc of a single head.
       const uint32_t x = fastdiv(p, a.head_div);
-      int found = 0;
       uint32_t pre;
       if (small) {
         const uint32_t before = inc - sum;
-        found = __popcll(__builtin_amdgcn_ballot_w64(before <= x));
-        pre = (uint32_t)__builtin_amdgcn_readlane((int)before, found - 1);
+        const int in = __popcll(__builtin_amdgcn_ballot_w64(before <= x)) - 1;
+        uint32_t past = 0, at_past = before;
+#pragma unroll
+        for (int j = 0; j < kSlice - 1; ++j) {
+          const bool over = before + upto[j] <= x;  // (beyond the slice: no, as no unit x)
+          past += over ? 1 : 0;
+          at_past = over ? before + upto[j] : at_past;
+        }
+        at.b = in * slice + (int)__builtin_amdgcn_readlane((int)past, in);
+        pre = (uint32_t)__builtin_amdgcn_readlane((int)at_past, in);
+        at.len = length_of(a, at.b);
+        at.units = units_of(at.len);
       } else {
+        int found = 0;
 #pragma unroll
         for (int j = 0; j < kWaves; ++j)
           found += __popcll(__builtin_amdgcn_ballot_w64(prefix[j * 64 + lane] <= x));
         pre = (uint32_t)__builtin_amdgcn_readfirstlane((int)prefix[found - 1]);
-      }
-      at.b = __builtin_amdgcn_readfirstlane((found - 1) * slice);
-      at.len = length_of(a, at.b);
-      at.units = units_of(at.len);
-      while (x - pre >= (uint32_t)at.units) {
-        pre += (uint32_t)at.units;
-        at.len = length_of(a, ++at.b);
+        at.b = __builtin_amdgcn_readfirstlane((found - 1) * slice);
+        at.len = length_of(a, at.b);
         at.units = units_of(at.len);
+        while (x - pre >= (uint32_t)at.units) {
+          pre += (uint32_t)at.units;
+          at.len = length_of(a, ++at.b);
+          at.units = units_of(at.len);
+        }
       }
       const uint32_t rem = p - pre * (uint32_t)Hc;
       at.hc = (int)(rem / (uint32_t)at.units);

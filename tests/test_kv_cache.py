@@ -461,7 +461,7 @@ def test_decode(gpu, lens, Hq, Hkv, bs):
 
 
 @pytest.mark.parametrize("B,longest,Hq,Hkv", [(70, 900, 32, 8), (1100, 40, 8, 2), (300, 200, 20, 1),
-                                              (65, 1500, 4, 4), (513, 33, 1, 1)])
+                                              (65, 1500, 4, 4), (513, 33, 1, 1), (250, 200, 8, 2)])
 def test_decode_many_requests(gpu, B, longest, Hq, Hkv):
     """More requests than a wave has lanes, more than a workgroup has threads, more segments than
     there are CUs: whole segments dealt out, and balanced shares; every seventh request empty."""
