@@ -30,6 +30,18 @@
 // within it to each wave. A wave finishes the segments that lie in its run;
 // its cut pieces meet in LDS, those that the workgroup's run cuts in the
 // workspace, where a second kernel folds them in order.
+//
+// What bounds it: HBM, at 136 bytes a token and kv-head. 32 requests of 8192 tokens
+// (32Q/8KV, blocks of 16: 286 MB) take 48.5 us, merge launch and all (5.9 TB/s); 64
+// ragged ones up to 32768 (64Q/8KV, blocks of 64: 1047 MB) 165 us (6.3 TB/s). The same
+// launches with the loads alone and no arithmetic took 47 and 164 us. 8 waves a
+// workgroup and one workgroup a CU, two waves a SIMD, with one unit (4352 bytes a
+// wave) in flight behind the one that is folded: two units ahead 2-5 % slower, 4
+// waves and two workgroups a CU 2-4 % slower at these sizes (and 3 % faster at 777
+// tokens), three waves a SIMD (168 registers) 5-25 % slower, one buffer whose
+// halves are refilled as they are used up 6-8 % slower. A unit costs a wave about
+// 2300 cycles (some 190 vector instructions with everything around them, 11 matrix
+// ones), half of what HBM takes to deliver the units of a CU's waves.
 #include <math.h>
 
 #include <algorithm>
@@ -881,8 +893,18 @@ struct Shape {
   int G, chunks, heads, capacity, workgroups, mode;
 };
 
-// Longest sequence, in units, that a workgroup takes alone.
-constexpr int kAloneUnits = 4 * kWaves;
+// Short sequences keep their segments whole: one launch, no merge, for shares
+// that are even only to a segment. Measured on MI355X, 32Q/8KV, block 16, whole
+// against balanced: tables of 1000 tokens, 1 to 64 full requests 9.1-17.4 us
+// against 10.8-18.1, 8 to 256 of U[1, 1000] 9.1-42.0 against 13.0-44.1; of 2000
+// tokens 8, 32 and 64 full requests 13.1, 15.4 and 28.8 against 13.0, 18.0 and
+// 28.9, 8 to 256 ragged ones 10.2-60.7 against 12.3-64.1, but a single request
+// (8 segments) 12.7 against 11.6 (at 1500 tokens 10.8 against 11.4); of 4000
+// tokens 1 and 8 full requests 20.0 and 20.8 against 11.7 and 15.6.
+constexpr int kWholeUnits = 64, kFewWholeUnits = 48;
+bool keep_whole(int64_t units, int64_t segments, int cus) {
+  return units <= (4 * segments >= cus ? kWholeUnits : kFewWholeUnits);
+}
 
 bool shape_of(int B, int Hq, int Hkv, int num_blocks, int block_size, int max_blocks,
               int num_workgroups, Shape& s) {
@@ -904,7 +926,7 @@ bool shape_of(int B, int Hq, int Hkv, int num_blocks, int block_size, int max_bl
   if (num_workgroups <= 0) {
     s.workgroups = gqa::device_cu_count();
     const int64_t segments = (int64_t)B * Hkv * s.chunks;
-    if ((cap + kUnit - 1) / kUnit <= kAloneUnits)
+    if (keep_whole((cap + kUnit - 1) / kUnit, segments, s.workgroups))
       s.mode = segments <= s.workgroups ? kPerSegment : kWhole;
     if (s.mode == kPerSegment) s.workgroups = (int)segments;
   }
