@@ -101,11 +101,19 @@ void check_written(const Rows& x) {
               " must not overlap itself");
 }
 
-void check_cache_apart(const Tensor& cache, const char* name, std::initializer_list<Rows> others) {
+// A contiguous cache as one row.
+Rows whole(const Tensor& cache, const char* name) {
   const int64_t elements = (int64_t)(cache.numel() * cache.element_size() + 1) / 2;
-  const Rows c{name, (int64_t)(reinterpret_cast<uintptr_t>(cache.data_ptr()) / 2), 1, 1, 0, 0,
-               elements};
-  for (const Rows& r : others) check_no_overlap(r, c);
+  return {name, (int64_t)(reinterpret_cast<uintptr_t>(cache.data_ptr()) / 2), 1, 1, 0, 0, elements};
+}
+
+void check_cache_apart(const Tensor& cache, const char* name, std::initializer_list<Rows> others) {
+  for (const Rows& r : others) check_no_overlap(r, whole(cache, name));
+}
+
+void check_aligned(const Tensor& t, const char* name, uintptr_t to) {
+  TORCH_CHECK(reinterpret_cast<uintptr_t>(t.data_ptr()) % to == 0, name, " must be ", to,
+              "-byte aligned");
 }
 
 struct Index {
@@ -169,6 +177,7 @@ void check_mxfp4(const Tensor& cache, const Tensor& like) {
   TORCH_CHECK(cache.dim() == 4 && cache.size(1) > 0 && cache.size(2) > 0 &&
                   cache.size(3) == KV_MXFP4_TILE_BYTES,
               "kv_cache must be [num_blocks, Hkv, block_size / 16, 2176]");
+  check_aligned(cache, "kv_cache", 16);
   check_same_device(cache, like);
 }
 
@@ -225,6 +234,8 @@ Tensor append(bool mx, const Tensor& q, const Tensor& k, const Tensor& v, const 
                 "k_cache and v_cache must have the same shape");
     check_same_device(k_cache, q);
     check_same_device(*v_cache, q);
+    check_aligned(k_cache, "k_cache", 16);
+    check_aligned(*v_cache, "v_cache", 16);
     a.k_cache = bf16(k_cache);
     a.v_cache = bf16(*v_cache);
     a.num_blocks = narrow(k_cache.size(0), "k_cache");
@@ -249,7 +260,7 @@ Tensor append(bool mx, const Tensor& q, const Tensor& k, const Tensor& v, const 
   check_cache_apart(k_cache, mx ? "kv_cache" : "k_cache", {rq, rk, rv, ro});
   if (!mx) {
     check_cache_apart(*v_cache, "v_cache", {rq, rk, rv, ro});
-    check_cache_apart(k_cache, "k_cache", {rows_of("v_cache", v_cache->view({1, -1}))});
+    check_cache_apart(k_cache, "k_cache", {whole(*v_cache, "v_cache")});
   }
   a.q = bf16(q), a.k = bf16(k), a.v = bf16(v), a.q_out = bf16(out);
   a.q_token_stride = rq.st, a.q_head_stride = rq.sh;
@@ -325,6 +336,7 @@ Tensor mla_append(Tensor q_pe, Tensor c_kv, Tensor k_pe, Tensor kv_cache, Tensor
   TORCH_CHECK(kv_cache.dim() == 4 && kv_cache.size(1) > 0 && kv_cache.size(2) == 1 &&
                   kv_cache.size(3) == kLatent + kRope,
               "kv_cache must be [num_blocks, block_size, 1, 576]");
+  check_aligned(kv_cache, "kv_cache", 16);
   check_same_device(kv_cache, q_pe);
   const Index ix = check_tokens(q_pe.size(0), block_table, seq_lens, cu_seqlens, positions, q_pe);
   kv_append_mla_args a{};

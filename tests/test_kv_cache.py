@@ -321,6 +321,61 @@ def test_append_special_values(gpu):
         assert np.array_equal(got.float().numpy(), x.float().numpy(), equal_nan=True)
 
 
+@pytest.mark.parametrize("Hq,Hkv,interleaved,rot", [(32, 8, False, 128), (7, 7, True, 64),
+                                                    (64, 4, False, 96)])
+def test_append_large_steps(gpu, Hq, Hkv, interleaved, rot):
+    """A prefill large enough for waves that take several heads (and several passes, MLA) gives the
+    bits of the same rows appended a few at a time, and what the oracle gives."""
+    news, past, bs = [1, 1700, 0, 333, 967], [5, 0, 9, 40, 1], 16
+    lens = [n + m for n, m in zip(news, past)]
+    cu, T, table, nb = make_step(news, lens, bs, seed=3, pad_rows=9)
+    gen = torch.Generator().manual_seed(Hq)
+    q, k, v = (normal(gen, T, h, D).to(gpu) for h in (Hq, Hkv, Hkv))
+    q_pe, c, k_pe = (normal(gen, T, *n).to(gpu) for n in ((20, 64), (512,), (64,)))
+    w, wc = (torch.rand(n, generator=gen).to(gpu) + 0.5 for n in (D, 512))
+    cs, cs64 = kv_cache.rotary_table(2000, rot), kv_cache.rotary_table(2000, 64)
+    table_d = table.to(gpu)
+
+    def caches():
+        return (torch.zeros(nb, bs, Hkv, D, dtype=torch.bfloat16, device=gpu),
+                torch.zeros(nb, bs, Hkv, D, dtype=torch.bfloat16, device=gpu),
+                kv_cache.new_mxfp4_cache(nb, bs, Hkv),
+                torch.zeros(nb, bs, 1, 576, dtype=torch.bfloat16, device=gpu))
+
+    def step(t0, t1, cu_step, lens_step, to):
+        how = dict(cu_seqlens=tensor(cu_step, gpu), interleaved=interleaved)
+        L = tensor(lens_step, gpu)
+        rows = [x[t0:t1] for x in (q, k, v)]
+        norms = dict(q_weight=w, k_weight=w)
+        return (kv_cache.kv_append(*rows, to[0], to[1], table_d, L, cs, **how, **norms),
+                kv_cache.kv_append_mxfp4(*rows, to[2], table_d, L, cs, **how, **norms),
+                kv_cache.mla_append(q_pe[t0:t1], c[t0:t1], k_pe[t0:t1], to[3], table_d, L, cs64,
+                                    c_weight=wc, **how))
+
+    one, few = caches(), caches()
+    whole = step(0, T, cu, lens, one)
+    parts = []
+    for t0 in range(0, T, 100):
+        t1 = min(t0 + 100, T)
+        inside = [max(0, min(t1, cu[b + 1]) - max(t0, cu[b])) for b in range(5)]
+        upto = [past[b] + max(0, min(t1, cu[b + 1]) - cu[b]) for b in range(5)]
+        parts.append(step(t0, t1, np.concatenate([[0], np.cumsum(inside)]), upto, few))
+    for a, b in zip(whole, zip(*parts)):
+        assert torch.equal(a, torch.cat(b))
+    for a, b in zip(one, few):
+        assert torch.equal(a, b)
+    where = ref.places(T, lens, cu)
+    some = [0, 1, 1000, 1700, 1701, 2033, 2034, 3000, T - 9, T - 1]
+    pos = [0 if where[t] is None else where[t][1] for t in some]
+    want, mag = turned(q[some].cpu(), w.cpu(), float(np.float32(1e-6)),
+                       ref.turn_rows(cs.cpu().numpy(), pos), interleaved)
+    pad = np.array([where[t] is None for t in some])
+    want[pad] = 0.0
+    assert pad.tolist() == [False] * 8 + [True] * 2
+    check_bf16(whole[0][some], want, mag, "q")
+    assert torch.equal(whole[0], whole[1])
+
+
 MLA_STEPS = ["one", "decode", "ragged", "prefill", "short"]
 
 
@@ -549,6 +604,64 @@ def test_decode_queries_that_are_not_finite(gpu):
         bad = torch.zeros(B, Hq, dtype=torch.bool, device=gpu)
         bad[0, 1] = bad[1, 0] = bad[1, Hq - 1] = True
         assert torch.isnan(got[bad]).all() and torch.isfinite(got[~bad]).all()
+
+
+def test_read_every_code_and_scale(gpu):
+    """All 16 codes under all 256 scale bytes: the nearest bf16 (the value itself but for the
+    overflow of the two largest scales), NaN under 255."""
+    rng = np.random.default_rng(12)
+    cache = rng.integers(0, 256, (32, 1, 1, 2176), dtype=np.uint8)
+    cache[..., 2048:] = rng.permutation(np.tile(np.arange(256, dtype=np.uint8), 16)).reshape(32, 1, 1,
+                                                                                         128)
+    k, v = kv_cache.kv_read_mxfp4(torch.from_numpy(cache).to(gpu),
+                                  torch.arange(32, dtype=torch.int32, device=gpu)[None],
+                                  tensor([512], gpu), tensor([0, 512], gpu), 512)
+    want = ref.mxfp4_rows(cache, np.arange(32), 512, 0)
+    for got, w in zip((k, v), want):
+        w = torch.from_numpy(w).float().bfloat16().float().numpy()
+        assert np.array_equal(got[:, 0].float().cpu().numpy(), w, equal_nan=True)
+
+
+def test_nothing_to_do(gpu):
+    """No tokens, no requests, no blocks: every call returns, and what it returns is empty or
+    zeros."""
+    q, k, v, kc, vc, table, lens, cs = decode_inputs(gpu)
+    mx = kv_cache.new_mxfp4_cache(3, 16, 2)
+    none = [t[:0] for t in (q, k, v)]
+    cu = torch.zeros(10, dtype=torch.int32, device=gpu)
+    was = kc.clone()
+    for args in ((table[:0], lens[:0], cs), (table, lens, cs, cu)):
+        assert kv_cache.kv_append(*none, kc, vc, *args).shape == (0, 8, D)
+        assert kv_cache.kv_append_mxfp4(*none, mx, *args).shape == (0, 8, D)
+    assert torch.equal(kc, was) and not mx.any()
+    # Rows with no request at all are padding.
+    assert not kv_cache.kv_append(q, k, v, kc, vc, table[:0], lens[:0], cs, cu[:1]).any()
+    assert torch.equal(kc, was)
+    # Caches without blocks take nothing; the queries turn all the same.
+    want = kv_cache.kv_append(q, k, v, kc, vc, table, lens, cs)
+    assert torch.equal(kv_cache.kv_append(q, k, v, kc[:0], vc[:0], table, lens, cs), want)
+    assert torch.equal(kv_cache.kv_append_mxfp4(q, k, v, mx[:0], table, lens, cs), want)
+    rows = kv_cache.kv_read_mxfp4(mx[:0], table, lens)
+    assert rows[0].shape == (9, 2, D) and not rows[0].any() and not rows[1].any()
+    assert kv_cache.kv_read_mxfp4(mx, table[:0], lens[:0])[0].shape == (0, 2, D)
+    assert kv_cache.kv_read_mxfp4(mx, table, lens, cu, 0)[1].shape == (0, 2, D)
+    pe, c = torch.zeros(0, 4, 64, dtype=torch.bfloat16, device=gpu), q.new_zeros(0, 512)
+    cache = torch.zeros(2, 64, 1, 576, dtype=torch.bfloat16, device=gpu)
+    assert kv_cache.mla_append(pe, c, q.new_zeros(0, 64), cache, table[:0], lens[:0],
+                               cs[:, :64].contiguous()).shape == (0, 4, 64)
+
+
+def test_misaligned_caches_are_refused(gpu):
+    q, k, v, kc, vc, table, lens, cs = decode_inputs(gpu)
+    odd = torch.zeros(kc.numel() + 1, dtype=torch.bfloat16, device=gpu)[1:].view(kc.shape)
+    with pytest.raises(RuntimeError, match="k_cache must be 16-byte aligned"):
+        kv_cache.kv_append(q, k, v, odd, vc, table, lens, cs)
+    mx = torch.zeros(4 * 2 * 2176 + 4, dtype=torch.uint8, device=gpu)[4:].view(4, 2, 1, 2176)
+    for call in (lambda: kv_cache.kv_append_mxfp4(q, k, v, mx, table, lens, cs),
+                 lambda: kv_cache.kv_read_mxfp4(mx, table, lens),
+                 lambda: kv_cache.gqa_decode_mxfp4(q, mx, table, lens, 0.1)):
+        with pytest.raises(RuntimeError, match="kv_cache must be 16-byte aligned"):
+            call()
 
 
 def test_decode_empty_batch_and_unaligned_q(gpu):
