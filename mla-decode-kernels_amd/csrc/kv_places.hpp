@@ -25,12 +25,16 @@ struct Search {
     const int s = (hi - lo + group - 1) / group;
     return s > 1 ? s : 1;
   }
-  // `count` of the probes were <= t.
-  KV_HD void narrow(int step, int count) {
+  // `count` of the probes were <= t. The entries next to the range go with it:
+  // entry lo - 1 becomes probe count - 1's if count > 0, entry hi probe count's if
+  // this says so.
+  KV_HD bool narrow(int step, int count) {
     const int end = lo + count * step;
-    if (end < hi) hi = end;
+    const bool below = end < hi;
+    if (below) hi = end;
     if (count > 0) lo += (count - 1) * step + 1;
     if (step == 1) hi = lo;
+    return below;
   }
   KV_HD int request() const { return lo - 1; }
 };

@@ -160,27 +160,38 @@ def places_lib(tmp_path_factory):
     src.write_text(r"""
 #include "kv_places.hpp"
 extern "C" int place(int t, int T, int B, const int* lens, const int* cu, int group, int* out) {
-  int b = t, first = t, next = t + 1, probes = 0;
+  int b = t, first = t, next = t + 1, len = 0, probes = 0;
   if (cu) {
     kv::Search s = kv::Search::begin(B);
+    first = cu[0];
     while (!s.done()) {
       if (++probes > 64) return -1;  // does not end
-      const int step = s.step(group);
+      const int step = s.step(group), lo = s.lo, hi = s.hi;
       int count = 0;
       for (int sub = 0; sub < group; ++sub) {
-        const int at = s.lo + sub * step;
-        if (at >= s.hi) continue;
+        const int at = lo + sub * step;
+        if (at >= hi) continue;
         if (at < 1 || at > B) return -2;  // outside cu_seqlens
         count += cu[at] <= t;
       }
-      s.narrow(step, count);
+      // What the lanes hand over, with the lanes that have it checked.
+      const int last = lo + (count - 1) * step, behind = lo + count * step;
+      if (count > 0) {
+        if (last >= hi) return -4;
+        first = cu[last];
+      }
+      if (s.narrow(step, count)) {
+        if (behind >= hi || count >= group) return -5;
+        next = cu[behind], len = lens[behind - 1];
+      }
     }
     b = s.request();
     if (b < 0 || b > B) return -3;
-    if (b < B) first = cu[b], next = cu[b + 1];
+  } else if (t < B) {
+    len = lens[t];
   }
   if (b >= B || t >= T) { out[2] = 0; return probes; }
-  const kv::Place p = kv::place_in(t, b, first, next, lens[b]);
+  const kv::Place p = kv::place_in(t, b, first, next, len);
   out[0] = p.b, out[1] = p.pos, out[2] = p.live;
   return probes;
 }
