@@ -63,7 +63,7 @@ extern "C" {
 #define KV_MXFP4_TILE_TOKENS 16
 #define KV_MXFP4_TILE_BYTES 2176
 
-/* Most new tokens (T) of a call. */
+/* Most new tokens (T) of a call (whose requests are at most 2^30). */
 #define KV_MAX_TOKENS (1 << 23)
 
 /* Types of a norm weight. */
@@ -126,8 +126,9 @@ GQA_DECODE_API int kv_append_mxfp4_launch(const kv_append_args* args, hipStream_
 
 /* The keys and values of the rows that an append with the same T, cu_seqlens,
  * seq_lens and block_table writes, as bf16 [T, Hkv, 128] (contiguous, 16-byte
- * aligned): every value of the 4-bit format is a bf16 value. (With seq_lens the
- * requests' lengths and cu_seqlens their running sum, the whole cache.) */
+ * aligned): every value of the 4-bit format is a bf16 value (but those of 2^128
+ * and more, under scale bytes 253 and 254, which read as infinities). With seq_lens
+ * the requests' lengths and cu_seqlens their running sum, the whole cache. */
 GQA_DECODE_API int kv_read_mxfp4_launch(const uint8_t* mxfp4_cache, const int* block_table,
                                         const int* seq_lens, const int* cu_seqlens,
                                         uint16_t* k_out, uint16_t* v_out, int T, int B, int Hkv,

@@ -3,14 +3,14 @@
 // the step's rows; and the read-back of rows of the 4-bit cache.
 //
 // What bounds them is the bytes, read once and written once, once there are enough
-// of them: 6358 tokens (32Q/8KV, half of each head turned) 180 MB in 36 us of GPU time,
-// 4.9 TB/s, the rate of a plain copy; below some 500 tokens the chain of latencies
+// of them: 7255 tokens (32Q/8KV, half of each head turned) 180 MB in 35 us of GPU time,
+// 5.1 TB/s, the rate of a plain copy; below some 500 tokens the chain of latencies
 // (request, length, block id, angles), 3-5 us. A wave takes four tokens, 16
 // lanes (a DPP row) each, 8 dims a lane, and walks heads: the tokens' places
 // and their angles (16 registers) are found once and serve every head. In
 // the 4-bit cache four tokens of a request, if they are aligned, are one whole
 // 256-byte line of value codes. The 4-bit append of 3880 tokens with norms moves 81 MB
-// in 23 us (3.5 TB/s): fp64 costs 2 us of them, the norms 2, the search for places 2.
+// in 23 us (3.5 TB/s): fp64 costs 2 us of them, the norms 2, the search for places 1.
 #include <type_traits>
 
 #include "kv_cache.h"
@@ -36,7 +36,6 @@ struct Turn {
 // How pairs lie: neighbours in a lane, 8 lanes apart (the halves of 128 dims: a
 // rotation by 8 within the DPP row, no LDS), or in lane `partner`.
 enum Pairs { kInside, kHalfRow, kPartner };
-
 
 // kLanes lanes hold a row of 8 kLanes dims, of which the first rot turn.
 template <int kLanes>
@@ -421,6 +420,7 @@ bool misaligned(const void* p, uintptr_t to) { return (reinterpret_cast<uintptr_
 // Sizes that every append and read shares.
 hipError_t check_sizes(int T, int B, bool ragged, int num_blocks, int block_size, int max_blocks) {
   if (T < 0 || T > KV_MAX_TOKENS || B < 0 || num_blocks < 0) return hipErrorInvalidValue;
+  if (B > (1 << 30)) return hipErrorInvalidValue;  // the search's steps fit 32 bits
   if (block_size < 1 || max_blocks < 1) return hipErrorInvalidValue;
   if (!ragged && T != B) return hipErrorInvalidValue;
   return hipSuccess;
@@ -466,7 +466,7 @@ int append(const kv_append_args* args, hipStream_t stream) {
   };
   // Heads a wave: with 4 a place is found for four rows, with 1 there are four times
   // as many waves to hide its latency. bf16, 32Q/8KV, norms: 128, 512 and 1024 tokens
-  // 3.6, 5.4 and 8.9 us with 1, 4.7, 5.5 and 7.9 with 4 (2 and 8 at 6358 tokens: 44.9
+  // 3.6, 5.4 and 8.9 us with 1, 4.7, 5.5 and 7.9 with 4 (2 and 8 at 7255 tokens: 44.9
   // and 42.2 us, with 4 41.7).
   if ((int64_t)groups * (a.Hq + 2 * a.Hkv) <= 8192)
     launch(std::integral_constant<int, 1>{});

@@ -9,6 +9,7 @@
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
 
+#include <cmath>
 #include <optional>
 
 #include "kv_cache.h"

@@ -81,6 +81,20 @@ def test_append_refuses(over):
     assert capi.kv_append_mxfp4_launch(append_args(**over), None) == INVALID
 
 
+def test_more_requests_than_the_search_counts():
+    over = dict(T=4, B=(1 << 30) + 1, cu_seqlens=SOME)
+    assert capi.kv_append_launch(append_args(**over), None) == INVALID
+    assert capi.kv_append_mxfp4_launch(append_args(**over), None) == INVALID
+    a = capi.KvAppendMlaArgs()
+    for n in ("q_pe", "c", "k_pe", "q_out", "kv_cache", "block_table", "seq_lens", "cos_sin"):
+        setattr(a, n, SOME)
+    a.h_q, a.num_blocks, a.block_size, a.max_blocks, a.table_rows = 16, 10, 64, 3, 100
+    a.T, a.B, a.cu_seqlens = 4, (1 << 30) + 1, SOME
+    assert capi.kv_append_mla_launch(a, None) == INVALID
+    args = [SOME, SOME, SOME, SOME, SOME, SOME, 4, (1 << 30) + 1, 2, 10, 16, 3, None]
+    assert capi.kv_read_mxfp4_launch(*args) == INVALID
+
+
 def test_append_refuses_caches():
     for over in (dict(k_cache=None), dict(v_cache=None), dict(k_cache=SOME + 8),
                  dict(v_cache=SOME + 2)):
