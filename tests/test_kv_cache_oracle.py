@@ -1,4 +1,4 @@
-"""CPU tests that pin oracle/kv_reference.py, the checker of the cache operators."""
+"""CPU tests that pin oracle/kv_reference.py, what the cache operators are compared with."""
 
 import numpy as np
 import pytest
