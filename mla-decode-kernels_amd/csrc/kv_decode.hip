@@ -11,8 +11,9 @@
 //          parts, q = 2^E (hi + lo / 16) with one E a head: a bf16 value has 8
 //          significant bits and e4m3 has 4, so the parts hold every value down
 //          to 2^-13 of the head's largest exactly, and the rest to 2^-21 of it.
-//          Groups of up to 8 q-heads put the hi parts into columns 0-7 and the
-//          lo parts into columns 8-15 of one instruction; wider ones take two.
+//          A group of up to 4 (8) q-heads has every head in four (two) columns, so
+//          that one instruction takes the hi parts in some and the lo parts in the
+//          others; wider ones take two.
 //   softmax on the C layout: lane (c, g) holds tokens 4g .. 4g+3 of each tile
 //          for column c.
 //   PV     O^T[128 dims x 16 cols] += V^T . P^T on 8 v_mfma_f32_16x16x32_bf16,
@@ -20,8 +21,11 @@
 //          second, which is where the scores lie (no data crosses lanes) and
 //          what a lane loads of the values: 8 dims 8c .. 8c+7 of those 8
 //          tokens. v_cvt_scalef32_pk_bf16_fp4 widens them exactly, scale and
-//          all. P enters as two bf16 parts as well, p = p_hi + p_lo (truncated:
-//          2^-15 relative), in columns 0-7 and 8-15 or in two products.
+//          all. P enters as three bf16 parts, the 24 bits of its fp32 value 8 at a
+//          time (nothing is cut off): a head's columns take different parts, so
+//          that 1 product does for up to 4 q-heads, 2 for up to 8 and 3 for 16.
+//          (Two truncated parts, 16 bits, took 1-4 % less and were off by up to
+//          2^-15.)
 //          The sum of the weights is one more product, with ones for V^T, so
 //          that the weights that are summed are those that were multiplied.
 //
@@ -49,7 +53,7 @@
 
 #include "gqa_launch.hpp"
 #include "kv_cache.h"
-#include "kv_common.hpp"
+#include "kv_decode.hpp"
 
 namespace {
 
@@ -60,9 +64,7 @@ using gqa::kNegInf;
 using gqa::wave_max;
 using gqa::wave_sum;
 using gqa::xor16_max;
-using gqa::xor16_sum;
 using gqa::xor32_max;
-using gqa::xor32_sum;
 
 typedef __bf16 bf16x8_t __attribute__((ext_vector_type(8)));
 typedef float f32x4_t __attribute__((ext_vector_type(4)));
@@ -74,19 +76,9 @@ constexpr int kUnit = 32;       // tokens a wave takes at a time
 constexpr int kWaves = 8;       // waves of a workgroup
 constexpr int kThreads = 64 * kWaves;
 static_assert((kWaves & (kWaves - 1)) == 0, "heads are dealt out by masks");
-constexpr int kPitch = 132;     // floats of a head's state: acc [128], m, l, pad
 constexpr int kMinUnits = 2;    // units a wave gets before another workgroup joins in
 
 constexpr int kSlice = 4;       // requests a lane keeps the prefix sums of (8 cost 512 requests 0.7 us)
-
-constexpr int kHasA = 1, kEndsA = 2, kHasZ = 4;  // pieces of a share (Record::flags)
-
-// A wave's or a workgroup's cut pieces: what they are, their first row of out
-// (request and q-head) and the number of its rows. (Rows and not segments: whoever
-// folds them has nothing to divide.)
-struct Record {
-  int flags, row_a, row_z, heads;  // heads: of A, and of Z from bit 8 on
-};
 
 // How the units are shared out.
 enum : int {
@@ -123,28 +115,28 @@ struct Unit {
   uint32_t ok;  // bit h: tile h lies in the cache
 };
 
-template <bool kWide>
 struct State {
   float m;         // running maximum of the column's raw scores
   f32x4_t o[8];    // o[j][e]: dim 32g + 8e + j of column c
   f32x4_t l;       // sum of the weights (four times the same)
 };
 
-template <bool kWide>
+// kCols: 4, 8 or 16, the smallest that holds the group's q-heads.
+template <int kCols>
 struct Query {
-  i32x8_t part[kWide ? 2 : 1];
-  int scale[kWide ? 2 : 1];
+  i32x8_t part[kCols < 16 ? 1 : 2];
+  int scale[kCols < 16 ? 1 : 2];
 };
 
-// The queries of heads h0 .. h0 + nh - 1 of request b, a head to each column:
-// lane (c, g), first 32 bytes: dims 16g .., then: dims 64 + 16g ...
+// The queries of heads h0 .. h0 + nh - 1 of request b, head i in columns i, i + kCols,
+// ..: lane (c, g), first 32 bytes: dims 16g .., then: dims 64 + 16g ...
 struct RawQuery {
   uint4 w[4];
 };
-template <bool kWide>
+template <int kCols>
 __device__ __forceinline__ RawQuery load_query(const DecodeArgs& a, int b, int h0, int nh, int c,
                                                int g) {
-  const int head = kWide ? c : (c & 7);
+  const int head = c & (kCols - 1);
   RawQuery r;
 #pragma unroll
   for (int part = 0; part < 4; ++part) {
@@ -167,8 +159,8 @@ __device__ __forceinline__ uint32_t xor32_umax(uint32_t x) {
 
 // The same as the B operand, in two e4m3 parts (the conversions divide by the
 // exponent of their scale).
-template <bool kWide>
-__device__ __forceinline__ Query<kWide> split_query(const RawQuery& r, uint32_t flip, int c) {
+template <int kCols>
+__device__ __forceinline__ Query<kCols> split_query(const RawQuery& r, uint32_t flip, int c) {
   // The largest magnitude of the head, as bf16 bits.
   u16x2_t most = {0, 0};
 #pragma unroll
@@ -185,7 +177,7 @@ __device__ __forceinline__ Query<kWide> split_query(const RawQuery& r, uint32_t 
   const int E = max((int)(top >> 7) - 127 - 7, -118);
   const float s = __uint_as_float((uint32_t)(127 + E) << 23);
   const float s16 = __uint_as_float((uint32_t)(123 + E) << 23);
-  Query<kWide> q;
+  Query<kCols> q;
   uint32_t hi[8], lo[8];
 #pragma unroll
   for (int w = 0; w < 8; ++w) {
@@ -203,7 +195,7 @@ __device__ __forceinline__ Query<kWide> split_query(const RawQuery& r, uint32_t 
                                                  s16, true);
     lo[w] = __builtin_bit_cast(uint32_t, l);
   }
-  if constexpr (kWide) {
+  if constexpr (kCols == 16) {
 #pragma unroll
     for (int w = 0; w < 8; ++w) {
       q.part[0][w] = (int)hi[w];
@@ -212,7 +204,7 @@ __device__ __forceinline__ Query<kWide> split_query(const RawQuery& r, uint32_t 
     q.scale[0] = top < 0x7f80u ? E + 127 : 255;
     q.scale[1] = top < 0x7f80u ? E + 123 : 255;
   } else {
-    const bool low = c >= 8;
+    const bool low = (c & kCols) != 0;
 #pragma unroll
     for (int w = 0; w < 8; ++w) q.part[0][w] = (int)(low ? lo[w] : hi[w]);
     q.scale[0] = top < 0x7f80u ? E + (low ? 123 : 127) : 255;
@@ -314,10 +306,23 @@ __device__ __forceinline__ uint32_t select_bits(uint32_t mask, uint32_t x, uint3
   return (x & mask) | (y & ~mask);
 }
 
+// x without the bits of it under `mask`, exactly.
+__device__ __forceinline__ float rest_of(float x, uint32_t mask) {
+  return x - __uint_as_float(__float_as_uint(x) & mask);
+}
+
+// The sum of a head's columns (rotations by 8 and by 4 within the row).
+template <int kCols>
+__device__ __forceinline__ float sum_columns(float x) {
+  if constexpr (kCols < 16) x += dpp_f32<0x128>(x);
+  if constexpr (kCols < 8) x += dpp_f32<0x124>(x);
+  return x;
+}
+
 // Fold a unit into the state.
-template <bool kWide>
-__device__ __forceinline__ void fold_unit(const Unit& u, const Mask& mask, const Query<kWide>& q,
-                                          float scale, int c, State<kWide>& st) {
+template <int kCols>
+__device__ __forceinline__ void fold_unit(const Unit& u, const Mask& mask, const Query<kCols>& q,
+                                          float scale, int c, State& st) {
   constexpr uint32_t kLow16 = 0x05040100u, kHigh16 = 0x07060302u;
   // Scale bytes to exponent fields; the bits around them do not count.
   float vs[8];
@@ -350,13 +355,13 @@ __device__ __forceinline__ void fold_unit(const Unit& u, const Mask& mask, const
     const int ks = (int)select_bits(mask.ks[h], u.ks[h], 127u);
     f32x4_t d = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(k, q.part[0], mask.bias[h], 4, 0, 0,
                                                                  ks, 0, q.scale[0]);
-    if constexpr (kWide)
+    if constexpr (kCols == 16)
       d = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(k, q.part[1], d, 4, 0, 0, ks, 0,
                                                            q.scale[1]);
 #pragma unroll
     for (int e = 0; e < 4; ++e)
-      // Columns c and c + 8 hold the two parts: a rotation by 8 within the row.
-      s[4 * h + e] = kWide ? d[e] : d[e] + dpp_f32<0x128>(d[e]);
+      // Columns c and c +- kCols hold the two parts: a rotation within the row.
+      s[4 * h + e] = kCols == 16 ? d[e] : d[e] + dpp_f32<0x120 + kCols % 16>(d[e]);
   }
   float mx = s[0];
 #pragma unroll
@@ -371,26 +376,32 @@ __device__ __forceinline__ void fold_unit(const Unit& u, const Mask& mask, const
     for (int j = 0; j < 8; ++j) st.o[j] *= alpha;
   }
   const float ms = st.m == kNegInf ? 0.f : st.m * scale;
-  uint32_t p[kWide ? 2 : 1][8];
-  const uint32_t low = kWide || c < 8 ? 0u : 0xffff0000u;
+  // The weights' parts: the upper 16 bits of each (truncated), then of what that
+  // left of them, an exact difference. kParts products; what a column gives to them:
+  //   kCols 4   columns 0-3 the first part, 4-7 the second, 8-11 the third, then none;
+  //   kCols 8   columns 0-7 the first, then none, 8-15 the second, then the third;
+  //   kCols 16  all columns one after the other.
+  constexpr uint32_t kUpper = 0xffff0000u;
+  constexpr int kParts = kCols == 4 ? 1 : kCols == 8 ? 2 : 3;
+  const uint32_t first = c >= kCols ? kUpper : 0u, second = c >= 12 ? ~0u : c >= 8 ? kUpper : 0u;
+  float p[kParts][8];
 #pragma unroll
   for (int e = 0; e < 8; ++e) {
     const float w = exp2_fast(fmaf(s[e], scale, -ms));
-    const uint32_t bits = __float_as_uint(w);
-    if constexpr (kWide) {
-      p[0][e] = bits;
-      p[1][e] = __float_as_uint(w - __uint_as_float(bits & 0xffff0000u));
-    } else {
-      p[0][e] = __float_as_uint(w - __uint_as_float(bits & low));
-    }
+    p[0][e] = kCols < 16 ? rest_of(w, first) : w;
+    if constexpr (kCols == 4) p[0][e] = rest_of(p[0][e], second);
+    if constexpr (kCols >= 8) p[1][e] = rest_of(p[0][e], kUpper);
+    if constexpr (kCols == 16) p[2][e] = rest_of(p[1][e], kUpper);
   }
-  bf16x8_t pb[kWide ? 2 : 1];
+  bf16x8_t pb[kParts];
 #pragma unroll
-  for (int i = 0; i < (kWide ? 2 : 1); ++i) {
+  for (int i = 0; i < kParts; ++i) {
+    const uint32_t some = kCols == 8 && i == 1 && c < 8 ? 0u : ~0u;
     u32x4 w;
 #pragma unroll
     for (int e = 0; e < 4; ++e)
-      w[e] = __builtin_amdgcn_perm(p[i][2 * e + 1], p[i][2 * e], kHigh16);
+      w[e] = some & __builtin_amdgcn_perm(__float_as_uint(p[i][2 * e + 1]),
+                                          __float_as_uint(p[i][2 * e]), kHigh16);
     pb[i] = __builtin_bit_cast(bf16x8_t, w);
   }
   const auto two_dims = [&](auto byte) {
@@ -398,7 +409,7 @@ __device__ __forceinline__ void fold_unit(const Unit& u, const Mask& mask, const
     u32x4 even, odd;
     pairs(byte, even, odd);
 #pragma unroll
-    for (int i = 0; i < (kWide ? 2 : 1); ++i) {
+    for (int i = 0; i < kParts; ++i) {
       st.o[j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, even), pb[i],
                                                         st.o[j], 0, 0, 0);
       st.o[j + 1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, odd),
@@ -407,7 +418,7 @@ __device__ __forceinline__ void fold_unit(const Unit& u, const Mask& mask, const
   };
   const u32x4 one = {0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u};
 #pragma unroll
-  for (int i = 0; i < (kWide ? 2 : 1); ++i)
+  for (int i = 0; i < kParts; ++i)
     st.l = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, one), pb[i], st.l, 0,
                                                    0, 0);
   two_dims(std::integral_constant<int, 0>{});
@@ -415,10 +426,6 @@ __device__ __forceinline__ void fold_unit(const Unit& u, const Mask& mask, const
   two_dims(std::integral_constant<int, 2>{});
   two_dims(std::integral_constant<int, 3>{});
 }
-
-// What a row is multiplied by in the end, 1 / l; a segment without a single token
-// gets zeros. (One quotient a lane: its fp32 rounding is nothing to bf16's.)
-__device__ __forceinline__ float inverse(float l) { return l == 0.f ? 0.f : 1.f / l; }
 
 // The q-heads of segment (b, hc): h0 .. h0 + the result - 1.
 __device__ __forceinline__ int heads_of(const DecodeArgs& a, int hc, int& h0) {
@@ -480,7 +487,7 @@ __device__ __forceinline__ uint32_t wave_prefix(uint32_t x) {
   return x + (lane >= 16 ? r0 : 0) + (lane >= 32 ? r1 : 0) + (lane >= 48 ? r2 : 0);
 }
 
-template <bool kWide>
+template <int kCols>
 __global__ __launch_bounds__(kThreads, 2) void kv_decode_kernel(DecodeArgs a) {
   extern __shared__ float slots[];  // [kWaves][2][heads][kPitch]
   __shared__ uint32_t prefix[kThreads];
@@ -511,7 +518,7 @@ __global__ __launch_bounds__(kThreads, 2) void kv_decode_kernel(DecodeArgs a) {
     // table row is there to its end, and an id is looked at before it is used):
     // one memory latency less in a launch that has little else.
     nh = heads_of(a, at.hc, h0);
-    raw = load_query<kWide>(a, at.b, h0, nh, c, g);
+    raw = load_query<kCols>(a, at.b, h0, nh, c, g);
     if (wave < units_of(a.capacity)) {
       next = find_unit(a, segment_of(a, at.b, at.hc, a.capacity), wave);
       load_unit(a, next, lanes, x0);
@@ -629,7 +636,7 @@ __global__ __launch_bounds__(kThreads, 2) void kv_decode_kernel(DecodeArgs a) {
     if (a.mode != kPerSegment) {
       // (The queries first: their conversion waits for no tile.)
       nh = heads_of(a, at.hc, h0);
-      raw = load_query<kWide>(a, at.b, h0, nh, c, g);
+      raw = load_query<kCols>(a, at.b, h0, nh, c, g);
       load_unit(a, next, lanes, x0);
     }
     next_unit(a, ahead, seg, next);
@@ -644,14 +651,14 @@ __global__ __launch_bounds__(kThreads, 2) void kv_decode_kernel(DecodeArgs a) {
         ends = wave == min(at.units, kWaves) - 1;
       }
       const int row = at.b * a.Hq + h0, heads = nh;
-      const Query<kWide> q = split_query<kWide>(raw, a.flip, c);
+      const Query<kCols> q = split_query<kCols>(raw, a.flip, c);
       at.left -= (uint32_t)k;
       if (at.left > 0) {  // the next segment's queries are on their way meanwhile
         next_segment(a, at);
         nh = heads_of(a, at.hc, h0);
-        raw = load_query<kWide>(a, at.b, h0, nh, c, g);
+        raw = load_query<kCols>(a, at.b, h0, nh, c, g);
       }
-      State<kWide> st;
+      State st;
       st.m = kNegInf;
       st.l = f32x4_t{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
@@ -665,7 +672,7 @@ __global__ __launch_bounds__(kThreads, 2) void kv_decode_kernel(DecodeArgs a) {
           set_mask(mask, x.rest, x.ok, c, g);
           unmasked = whole;
         }
-        fold_unit<kWide>(x, mask, q, a.scale, c, st);
+        fold_unit<kCols>(x, mask, q, a.scale, c, st);
         return --k == 0;
       };
       while (true) {
@@ -675,12 +682,12 @@ __global__ __launch_bounds__(kThreads, 2) void kv_decode_kernel(DecodeArgs a) {
         }
         if (step(x1, x0)) break;
       }
-      if constexpr (!kWide) {
-        st.l += f32x4_t{dpp_f32<0x128>(st.l[0]), 0.f, 0.f, 0.f};
+      if constexpr (kCols < 16) {
+        st.l[0] = sum_columns<kCols>(st.l[0]);
 #pragma unroll
         for (int j = 0; j < 8; ++j)
 #pragma unroll
-          for (int e = 0; e < 4; ++e) st.o[j][e] += dpp_f32<0x128>(st.o[j][e]);
+          for (int e = 0; e < 4; ++e) st.o[j][e] = sum_columns<kCols>(st.o[j][e]);
       }
       const float l = st.l[0];
       if (starts && ends) {
@@ -813,82 +820,6 @@ __global__ __launch_bounds__(kThreads, 2) void kv_decode_kernel(DecodeArgs a) {
   }
 }
 
-// Segments cut between workgroups: the workgroup whose first piece ends one
-// folds it, from the one whose last piece starts it. A wave to a head; a row of
-// 16 lanes takes every fourth piece, 8 dims a lane, with a state of its own, and
-// the four rows meet at the end. One chain of latencies (records, states, the
-// sum over the rows), so what shortens it is few instructions on a wave that has
-// its SIMD to itself. Against 16 waves on one CU that share a segment's heads and
-// pieces and meet in LDS: 4 requests of 2048 tokens 11.4 us in all for 12.3, a
-// ragged batch of 64 (64Q/8KV) 167.6 for 168.8; one request of 32768 (32 pieces to
-// a segment) 17.0 for 16.6.
-struct MergeArgs {
-  const Record* records;
-  const float* states;
-  uint16_t* out;
-  uint32_t slot_floats;
-};
-constexpr int kMergeWaves = 4;
-__global__ __launch_bounds__(64 * kMergeWaves) void kv_decode_merge_kernel(MergeArgs a) {
-  const int wg = blockIdx.x, lane = threadIdx.x & 63;
-  // Lane i reads record wg - i: the workgroup's own, and those in front.
-  const Record r = a.records[max(wg - lane, 0)];
-  const int flags = __builtin_amdgcn_readfirstlane(r.flags);
-  const int h = (int)blockIdx.y * kMergeWaves +
-                __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
-  if ((flags & (kHasA | kEndsA)) != (kHasA | kEndsA)) return;
-  if (h >= __builtin_amdgcn_readfirstlane(r.heads)) return;
-  const int row = __builtin_amdgcn_readfirstlane(r.row_a) + h;
-  uint64_t hit = __builtin_amdgcn_ballot_w64(lane > 0 && lane <= wg && (r.flags & kHasZ) != 0);
-  int base = wg;
-  while (!hit) {
-    base -= 64;
-    if (base < 0) return;
-    hit = __builtin_amdgcn_ballot_w64(lane <= base &&
-                                      (a.records[max(base - lane, 0)].flags & kHasZ) != 0);
-  }
-  const int from = base - (int)__builtin_ctzll(hit);
-  // (Shares go to the first workgroups, so all from `from` to wg have a piece: a Z,
-  // then As.)
-  const int n = wg - from + 1, i = lane & 15;
-  const float* const states = a.states + (size_t)from * 2 * a.slot_floats + h * kPitch;
-  struct Piece {
-    float2 ml;
-    f32x4_t v[2];
-  };
-  const auto load = [&](int p) {
-    const float* s =
-        states + (size_t)(p == 0 ? 1u : 2 * (uint32_t)min(p, n - 1)) * a.slot_floats;
-    return Piece{*reinterpret_cast<const float2*>(s + kDim),
-                 {reinterpret_cast<const f32x4_t*>(s + 8 * i)[0],
-                  reinterpret_cast<const f32x4_t*>(s + 8 * i)[1]}};
-  };
-  float M = kNegInf, L = 0.f;
-  f32x4_t x[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
-  int p = lane >> 4;
-  Piece next = load(p), after = load(p + 4);
-  for (int p0 = 0; p0 < n; p0 += 4, p += 4) {
-    const Piece now = next;
-    next = after;
-    after = load(p + 8);
-    if (p >= n) break;  // (these rows are done)
-    const float m = fmaxf(M, now.ml.x), ref = m == kNegInf ? 0.f : m;
-    const float old = exp2_fast(M - ref), f = exp2_fast(now.ml.x - ref);
-    M = m;
-    L = fmaf(L, old, now.ml.y * f);
-    x[0] = x[0] * old + now.v[0] * f;
-    x[1] = x[1] * old + now.v[1] * f;
-  }
-  const float top = xor32_max(xor16_max(M));
-  const float f = M == kNegInf ? 0.f : exp2_fast(M - top);
-  L = xor32_sum(xor16_sum(L * f));
-  const float inv = inverse(L);
-  float y[8];
-#pragma unroll
-  for (int e = 0; e < 8; ++e) y[e] = xor32_sum(xor16_sum(x[e >> 2][e & 3] * f)) * inv;
-  if (lane < 16) reinterpret_cast<uint4*>(a.out + (size_t)row * kDim)[i] = pack8(y);
-}
-
 struct Shape {
   int G, chunks, heads, capacity, workgroups, mode;
 };
@@ -998,7 +929,9 @@ extern "C" int kv_decode_mxfp4_launch(const uint16_t* q, const uint8_t* mxfp4_ca
   a.flip = scale < 0.f ? 0x80008000u : 0u;
   a.mode = s.mode;
   const size_t lds = (size_t)kWaves * 2 * s.heads * kPitch * sizeof(float);
-  const auto kernel = s.G > 8 ? kv_decode_kernel<true> : kv_decode_kernel<false>;
+  const auto kernel = s.G > 8   ? kv_decode_kernel<16>
+                      : s.G > 4 ? kv_decode_kernel<8>
+                                : kv_decode_kernel<4>;
   if (lds > 65536) {  // more than the default share of a CU's 160 KiB
     const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel),
                                              hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
@@ -1008,7 +941,5 @@ extern "C" int kv_decode_mxfp4_launch(const uint16_t* q, const uint8_t* mxfp4_ca
   hipError_t e = hipGetLastError();
   if (e != hipSuccess || s.mode != kBalanced) return e;
   const MergeArgs m{a.records, a.states, out, (uint32_t)s.heads * kPitch};
-  kv_decode_merge_kernel<<<dim3(s.workgroups, (s.heads + kMergeWaves - 1) / kMergeWaves),
-                           64 * kMergeWaves, 0, stream>>>(m);
-  return hipGetLastError();
+  return launch_decode_merge(m, s.workgroups, s.heads, stream);
 }

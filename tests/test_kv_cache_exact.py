@@ -1,0 +1,154 @@
+"""How exact the attention over the 4-bit cache is, beyond what the output's rounding
+hides (tests/test_kv_cache.py has the tolerances of arbitrary inputs).
+
+The inputs make the scores exact in fp32: queries are small integers times a power
+of two, keys multiples of a quantum, so that every product and sum of a score is a
+multiple of one quantum and fits 24 bits, whatever the order of the sum. What is
+left, for requests of up to 4 tokens and scores whose differences stay below 2^A in
+the exponent, relative to the sum of weight times |value|:
+  a weight: the scale times log2(e) (two roundings, 2^-23) and the fma (2^-24), times
+    A ln 2, and the exponential, 2^-23 (the maximum's rounding is common to all);
+    for numerator and denominator both;
+  the sums: a weight in up to 3 parts whose products are exact, 12 additions and 2
+    between columns, 2^-23 each, for both;
+  quotient and product: 2 * 2^-23.
+The output is then rounded to the nearest bf16 value: half its own step."""
+
+import math
+
+import numpy as np
+import pytest
+import torch
+
+import kv_cache
+from oracle import kv_reference as ref
+
+D = 128
+A = 4.0
+TOL = (2 * (1.5 * A * math.log(2) + 1) + 2 * 14 + 2) * 2.0 ** -23
+
+
+def half_step(x):
+    """Half the distance of the bf16 values around |x| (normal ones)."""
+    return 2.0 ** (np.floor(np.log2(np.maximum(np.abs(x), 2.0 ** -126))) - 8)
+
+
+def check_exact(got, want, mass, tol=TOL):
+    over = tol * mass
+    bad = ~(np.abs(got - want) <= half_step(np.abs(want) + over) + over)
+    assert not bad.any(), f"{bad.sum()} of {bad.size}"
+
+
+def exact_inputs(seed, B, Hq, Hkv, bs=16):
+    """Requests of 2 to 4 tokens: (q [B, Hq, 128] float64, cache, table, lengths, scale)."""
+    rng = np.random.default_rng(seed)
+    cache = rng.integers(0, 256, (B, Hkv, bs // 16, 2176), dtype=np.uint8)
+    cache[..., 2048:2112] = rng.integers(126, 129, (B, Hkv, bs // 16, 64), dtype=np.uint8)
+    cache[..., 2112:] = rng.integers(120, 134, (B, Hkv, bs // 16, 64), dtype=np.uint8)
+    q = rng.integers(-8, 9, (B, Hq, D)).astype(np.float64)
+    lens = [2 + b % 3 for b in range(B)]
+    table = np.arange(B)[:, None].astype(np.int32)
+    # Scores: multiples of 0.25 below 128 * 8 * 12; their differences times scale and
+    # log2(e) below A.
+    most = 0.0
+    for b, n in enumerate(lens):
+        for h in range(Hq):
+            s = ref.mxfp4_rows(cache, table[b], n, h // (Hq // Hkv))[0] @ q[b, h]
+            most = max(most, s.max() - s.min())
+    scale = 2.0 ** math.floor(math.log2(A / (most * math.log2(math.e))))
+    return q, cache, table, lens, scale
+
+
+def model(q, cache, table, lens, scale, parts, heads_per_kv):
+    """The attention with fp32 weights cut to `parts` (how many bits each keeps; None: whole),
+    rounded to bf16."""
+    B, Hq, _ = q.shape
+    out = np.zeros((B, Hq, D))
+    for b in range(B):
+        for h in range(Hq):
+            k, v, _ = ref.mxfp4_rows(cache, table[b], lens[b], h // heads_per_kv)
+            s = k @ q[b, h] * scale
+            w = np.exp(s - s.max()).astype(np.float32)
+            if parts is not None:
+                rest, total = w.copy(), np.zeros(len(w))
+                for _ in range(parts):
+                    p = (rest.view(np.uint32) & np.uint32(0xffff0000)).view(np.float32)
+                    total, rest = total + p, rest - p
+                w = total
+            out[b, h] = (w.astype(np.float64) @ v) / w.astype(np.float64).sum()
+    return torch.from_numpy(out).bfloat16().double().numpy()
+
+
+def test_the_check_tells_weights_of_fewer_bits():
+    q, cache, table, lens, scale = exact_inputs(0, 24, 8, 2)
+    want, mass, _, _ = ref.mxfp4_attention(q, cache, table, lens, scale)
+    for parts in (None, 3):
+        check_exact(model(q, cache, table, lens, scale, parts, 4), want, mass)
+    for got in (model(q, cache, table, lens, scale, 2, 4), model(q, cache, table, lens, scale, 1, 4),
+                np.zeros_like(want), 2 * want):
+        with pytest.raises(AssertionError):
+            check_exact(got, want, mass)
+
+
+def run(gpu, q, cache, table, lens, scale, **how):
+    qt = torch.from_numpy(q).bfloat16()
+    assert np.array_equal(qt.double().numpy(), q)
+    index = lambda x: torch.as_tensor(np.asarray(x), dtype=torch.int32).to(gpu)  # noqa: E731
+    out = kv_cache.gqa_decode_mxfp4(qt.to(gpu), torch.from_numpy(cache).to(gpu), index(table),
+                                    index(lens), scale, **how)
+    return out.double().cpu().numpy()
+
+
+GROUPS = [(2, 2), (8, 2), (4, 1), (5, 1), (16, 2), (9, 1), (32, 2), (20, 1)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("Hq,Hkv", GROUPS)
+def test_weights_keep_their_24_bits(gpu, Hq, Hkv):
+    q, cache, table, lens, scale = exact_inputs(Hq, 48, Hq, Hkv)
+    want, mass, _, _ = ref.mxfp4_attention(q, cache, table, lens, scale)
+    for how in ({}, {"num_workgroups": 5}):
+        check_exact(run(gpu, q, cache, table, lens, scale, **how), want, mass)
+
+
+# Rounding errors that spread evenly over half a step, 2^-8 of a value at most: 2^-8 / sqrt(3)
+# of the outputs in the 2-norm (less, as values lie all over a step's binade).
+NORM = 2.0 ** -8 / math.sqrt(3)
+
+
+def ordinary_inputs(seed, lens, Hq, Hkv, bs=16):
+    """Normal queries over random codes, scores of a few units: (q, cache, table, scale)."""
+    rng = np.random.default_rng(seed)
+    blocks = [-(-n // bs) for n in lens]
+    cache = rng.integers(0, 256, (sum(blocks), Hkv, bs // 16, 2176), dtype=np.uint8)
+    cache[..., 2048:] = rng.integers(125, 128, cache[..., 2048:].shape, dtype=np.uint8)
+    table = np.full((len(lens), max(blocks)), -1, dtype=np.int32)
+    at = 0
+    for b, n in enumerate(blocks):
+        table[b, :n] = np.arange(at, at + n)
+        at += n
+    q = torch.from_numpy(rng.normal(size=(len(lens), Hq, D))).bfloat16().double().numpy()
+    return q, cache, table, D ** -0.5
+
+
+def off(got, want):
+    return np.linalg.norm(got - want) / np.linalg.norm(want)
+
+
+def test_the_norm_tells_mistakes():
+    lens = [300, 77]
+    q, cache, table, scale = ordinary_inputs(3, lens, 4, 1)
+    want, _, _, _ = ref.mxfp4_attention(q, cache, table, lens, scale)
+    assert off(model(q, cache, table, lens, scale, None, 4), want) < NORM
+    for got in (model(q, cache, table, lens, scale, 1, 4), np.zeros_like(want), 2 * want):
+        assert off(got, want) > NORM
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("Hq,Hkv", GROUPS)
+def test_ordinary_batches(gpu, Hq, Hkv):
+    lens = [2000, 1, 333, 640, 77, 0, 1500]
+    q, cache, table, scale = ordinary_inputs(Hq, lens, Hq, Hkv)
+    want, _, _, _ = ref.mxfp4_attention(q, cache, table, lens, scale)
+    for how in ({}, {"num_workgroups": 37}):
+        assert off(run(gpu, q, cache, table, lens, scale, **how), want) < NORM
