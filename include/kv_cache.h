@@ -166,9 +166,11 @@ GQA_DECODE_API int kv_append_mla_launch(const kv_append_mla_args* args, hipStrea
 /* Single-token GQA decode over the 4-bit cache:
  *   out[b, h, :] = softmax_t(scale * <q[b, h, :], K_b[t, kv(h), :]>) . V_b[t, kv(h), :]
  * over t < min(seq_lens[b], max_blocks * block_size), kv(h) = h / (Hq / Hkv),
- * with K and V the values that the cache's codes stand for. q and out
- * [B, Hq, 128] bf16, contiguous; q, out and the cache 16-byte aligned; out must
- * not overlap q. A
+ * with K and V the values that the cache's codes stand for (V as bf16: of 2^128
+ * and more as infinities), in fp32 arithmetic of exact products, rounded once to
+ * bf16. (Units of 32 tokens that hold a key of scale byte 253 or 254 take their
+ * scores to some 14 bits of the largest product only.) q and out [B, Hq, 128] bf16,
+ * contiguous; q, out and the cache 16-byte aligned; out must not overlap q. A
  * request of length 0 gets zeros. Tokens in blocks whose id is outside
  * [0, num_blocks) are left out (a request with no other token gets zeros).
  * B * ceil(max_blocks * block_size / 32) * Hkv * ceil(Hq / Hkv / 16) is at most

@@ -5,15 +5,17 @@
 // and of value codes a lane and tile) and already in the matrix cores' operand
 // layouts. A unit, with lane l = (c, g) = (l % 16, l / 16):
 //
-//   QK^T   S[16 tok x 16 cols] = K . Q^T on v_mfma_scale_f32_16x16x128_f8f6f4:
-//          A = the key codes as they lie in the cache (lane: token c, dims
-//          32g .. +32) with their scale bytes, B = the queries in two e4m3
-//          parts, q = 2^E (hi + lo / 16) with one E a head: a bf16 value has 8
-//          significant bits and e4m3 has 4, so the parts hold every value down
-//          to 2^-13 of the head's largest exactly, and the rest to 2^-21 of it.
-//          A group of up to 4 (8) q-heads has every head in four (two) columns, so
-//          that one instruction takes the hi parts in some and the lo parts in the
-//          others; wider ones take two.
+//   QK^T   S[16 tok x 16 cols] = K . Q^T on 4 v_mfma_f32_16x16x32_bf16: A = the key
+//          codes (lane: token c, dims 32g .. +32, 8 of them an instruction) widened
+//          exactly by v_cvt_scalef32_pk_bf16_fp4, scale and all, B = the queries as
+//          they are. Products are exact and their sums fp32's (off by 8e-8 of the sum
+//          of magnitudes at most, measured). v_mfma_scale_f32_16x16x128_f8f6f4 would
+//          take codes and scales as they lie in the cache and half the time, but it
+//          wants the queries in e4m3 parts, whose lower ends get lost, and adds up
+//          neighbouring products with some 14 bits below the largest (off by up to
+//          1e-4 of the sum of magnitudes, measured). It is left for units with keys
+//          of scale bytes 253 and 254, whose larger codes are past bf16's range.
+//          Groups of up to 4 (8) q-heads have every head in four (two) columns.
 //   softmax on the C layout: lane (c, g) holds tokens 4g .. 4g+3 of each tile
 //          for column c.
 //   PV     O^T[128 dims x 16 cols] += V^T . P^T on 8 v_mfma_f32_16x16x32_bf16,
@@ -36,16 +38,17 @@
 // workspace, where a second kernel folds them in order.
 //
 // What bounds it: HBM, at 136 bytes a token and kv-head. 32 requests of 8192 tokens
-// (32Q/8KV, blocks of 16: 286 MB) take 48.5 us, merge launch and all (5.9 TB/s); 64
-// ragged ones up to 32768 (64Q/8KV, blocks of 64: 1047 MB) 165 us (6.3 TB/s). The same
+// (32Q/8KV, blocks of 16: 286 MB) take 49.3 us, merge launch and all (5.8 TB/s); 64
+// ragged ones up to 32768 (64Q/8KV, blocks of 64: 1047 MB) 180 us (5.8 TB/s). The same
 // launches with the loads alone and no arithmetic took 47 and 164 us. 8 waves a
 // workgroup and one workgroup a CU, two waves a SIMD, with one unit (4352 bytes a
-// wave) in flight behind the one that is folded: two units ahead 2-5 % slower, 4
+// wave) in flight behind the one that is folded: two units ahead 2-10 % slower, 4
 // waves and two workgroups a CU 2-4 % slower at these sizes (and 3 % faster at 777
 // tokens), three waves a SIMD (168 registers) 5-25 % slower, one buffer whose
-// halves are refilled as they are used up 6-8 % slower. A unit costs a wave about
-// 2300 cycles (some 190 vector instructions with everything around them, 11 matrix
-// ones), half of what HBM takes to deliver the units of a CU's waves.
+// halves are refilled as they are used up 6-8 % slower. A unit costs a wave some 220
+// vector instructions with everything around them and 17, 26 or 35 matrix ones
+// (groups of up to 4, 8, 16 q-heads); what the two waves of a SIMD do not overlap of
+// them is what the wider groups lose.
 #include <math.h>
 
 #include <algorithm>
@@ -121,15 +124,13 @@ struct State {
   f32x4_t l;       // sum of the weights (four times the same)
 };
 
-// kCols: 4, 8 or 16, the smallest that holds the group's q-heads.
-template <int kCols>
 struct Query {
-  i32x8_t part[kCols < 16 ? 1 : 2];
-  int scale[kCols < 16 ? 1 : 2];
+  bf16x8_t part[4];  // as RawQuery
 };
 
 // The queries of heads h0 .. h0 + nh - 1 of request b, head i in columns i, i + kCols,
-// ..: lane (c, g), first 32 bytes: dims 16g .., then: dims 64 + 16g ...
+// .. (kCols: 4, 8 or 16, the smallest that holds the group's q-heads): lane (c, g) has
+// dims 32g + 8i .. +8 in w[i].
 struct RawQuery {
   uint4 w[4];
 };
@@ -143,7 +144,7 @@ __device__ __forceinline__ RawQuery load_query(const DecodeArgs& a, int b, int h
     r.w[part] = make_uint4(0, 0, 0, 0);
     if (head < nh)
       r.w[part] = *reinterpret_cast<const uint4*>(
-          a.q + ((size_t)b * a.Hq + h0 + head) * kDim + (part >> 1) * 64 + 16 * g + 8 * (part & 1));
+          a.q + ((size_t)b * a.Hq + h0 + head) * kDim + 32 * g + 8 * part);
   }
   return r;
 }
@@ -157,59 +158,73 @@ __device__ __forceinline__ uint32_t xor32_umax(uint32_t x) {
   return max((uint32_t)p[0], (uint32_t)p[1]);
 }
 
-// The same as the B operand, in two e4m3 parts (the conversions divide by the
-// exponent of their scale).
-template <int kCols>
-__device__ __forceinline__ Query<kCols> split_query(const RawQuery& r, uint32_t flip, int c) {
-  // The largest magnitude of the head, as bf16 bits.
+// The same as the B operands. A lane with an infinity gets NaN, so that its head's
+// result is NaN whatever the keys are.
+__device__ __forceinline__ Query query_operands(const RawQuery& r, uint32_t flip) {
   u16x2_t most = {0, 0};
+  Query q;
 #pragma unroll
   for (int part = 0; part < 4; ++part) {
-    const uint32_t w[4] = {r.w[part].x, r.w[part].y, r.w[part].z, r.w[part].w};
+    const u32x4 w = {r.w[part].x, r.w[part].y, r.w[part].z, r.w[part].w};
 #pragma unroll
     for (int i = 0; i < 4; ++i)
       most = __builtin_elementwise_max(most, __builtin_bit_cast(u16x2_t, w[i] & 0x7fff7fffu));
+    q.part[part] = __builtin_bit_cast(bf16x8_t, w ^ flip);
   }
-  uint32_t top = max((uint32_t)most.x, (uint32_t)most.y);
+  if (max((uint32_t)most.x, (uint32_t)most.y) >= 0x7f80u) q.part[0][0] = (__bf16)__builtin_nanf("");
+  return q;
+}
+
+// Raw scores of two tiles by the scaled instruction, which knows no keys past its
+// range: queries in two e4m3 parts, q = 2^E (hi + lo / 16) with one E a head.
+__device__ __forceinline__ void far_scores(const Query& q, const uint4 (&k)[2],
+                                           const uint32_t (&ks)[2], const f32x4_t (&bias)[2],
+                                           f32x4_t (&d)[2]) {
+  // Its B operand: lane (c, g) holds dims 16g .. +16, then 64 + 16g .. +16.
+  uint32_t w[16];
+  uint32_t top = 0;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const uint32_t x = __builtin_bit_cast(u32x4, q.part[i >> 2])[i & 3];
+    const uint32_t y = __builtin_bit_cast(u32x4, q.part[2 + (i >> 2)])[i & 3];
+    const auto odd = __builtin_amdgcn_permlane16_swap(x, y, false, false);
+    const auto half = __builtin_amdgcn_permlane32_swap(odd[0], odd[1], false, false);
+    w[i] = half[0];
+    w[8 + i] = half[1];
+    top = max(max(top, w[i] & 0x7fffu), w[i] >> 16 & 0x7fffu);
+    top = max(max(top, w[8 + i] & 0x7fffu), w[8 + i] >> 16 & 0x7fffu);
+  }
   top = xor32_umax(xor16_umax(top));
-  // E puts it into [128, 256); e4m3 ends at 448. (A head that holds an infinity
-  // or NaN gets the scale NaN.)
+  // E puts the largest into [128, 256); e4m3 ends at 448. (The conversions divide by
+  // the exponent of their scale; a head with a NaN gets the scale NaN.)
   const int E = max((int)(top >> 7) - 127 - 7, -118);
   const float s = __uint_as_float((uint32_t)(127 + E) << 23);
   const float s16 = __uint_as_float((uint32_t)(123 + E) << 23);
-  Query<kCols> q;
-  uint32_t hi[8], lo[8];
+  i32x8_t hi, lo;
 #pragma unroll
-  for (int w = 0; w < 8; ++w) {
-    const uint4& four = r.w[w >> 1];
-    const uint32_t x[2] = {(w & 1 ? four.z : four.x) ^ flip, (w & 1 ? four.w : four.y) ^ flip};
+  for (int i = 0; i < 8; ++i) {
+    const uint32_t x[2] = {w[2 * i], w[2 * i + 1]};
     i16x2_t h = {0, 0}, l = {0, 0};
     h = __builtin_amdgcn_cvt_scalef32_pk_fp8_bf16(h, __builtin_bit_cast(bf16x2_t, x[0]), s, false);
     h = __builtin_amdgcn_cvt_scalef32_pk_fp8_bf16(h, __builtin_bit_cast(bf16x2_t, x[1]), s, true);
-    hi[w] = __builtin_bit_cast(uint32_t, h);
-    const f32x2_t b0 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(hi[w], s, false);
-    const f32x2_t b1 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(hi[w], s, true);
+    hi[i] = __builtin_bit_cast(int, h);
+    const f32x2_t b0 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(hi[i], s, false);
+    const f32x2_t b1 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(hi[i], s, true);
     l = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(l, bf16_lo(x[0]) - b0[0], bf16_hi(x[0]) - b0[1],
                                                  s16, false);
     l = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(l, bf16_lo(x[1]) - b1[0], bf16_hi(x[1]) - b1[1],
                                                  s16, true);
-    lo[w] = __builtin_bit_cast(uint32_t, l);
+    lo[i] = __builtin_bit_cast(int, l);
   }
-  if constexpr (kCols == 16) {
+  const int scale_hi = top < 0x7f80u ? E + 127 : 255, scale_lo = top < 0x7f80u ? E + 123 : 255;
 #pragma unroll
-    for (int w = 0; w < 8; ++w) {
-      q.part[0][w] = (int)hi[w];
-      q.part[1][w] = (int)lo[w];
-    }
-    q.scale[0] = top < 0x7f80u ? E + 127 : 255;
-    q.scale[1] = top < 0x7f80u ? E + 123 : 255;
-  } else {
-    const bool low = (c & kCols) != 0;
-#pragma unroll
-    for (int w = 0; w < 8; ++w) q.part[0][w] = (int)(low ? lo[w] : hi[w]);
-    q.scale[0] = top < 0x7f80u ? E + (low ? 123 : 127) : 255;
+  for (int h = 0; h < 2; ++h) {
+    const i32x8_t a = {(int)k[h].x, (int)k[h].y, (int)k[h].z, (int)k[h].w, 0, 0, 0, 0};
+    d[h] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, hi, bias[h], 4, 0, 0, (int)ks[h], 0,
+                                                            scale_hi);
+    d[h] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, lo, d[h], 4, 0, 0, (int)ks[h], 0,
+                                                            scale_lo);
   }
-  return q;
 }
 
 // Block ids through the constant address space: scalar loads, which do not
@@ -281,7 +296,7 @@ __device__ __forceinline__ void load_unit(const DecodeArgs& a, const Spot& s, co
 // What takes tokens out of a unit, in registers that stay the same while units
 // are whole: the C operand of QK^T (-infinity for a token that does not count),
 // and bytes that hide the scales of those tokens, which may be anything (255
-// would make them NaN), behind a scale of 1.
+// would make them NaN), behind the smallest one.
 struct Mask {
   f32x4_t bias[2];
   uint32_t ks[2], vs[2];
@@ -306,6 +321,16 @@ __device__ __forceinline__ uint32_t select_bits(uint32_t mask, uint32_t x, uint3
   return (x & mask) | (y & ~mask);
 }
 
+// Eight codes of one scale (exact: a code has two significant bits).
+__device__ __forceinline__ bf16x8_t widen8(uint32_t codes, float by) {
+  const u32x4 w = {
+      __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(codes, by, 0)),
+      __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(codes, by, 1)),
+      __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(codes, by, 2)),
+      __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(codes, by, 3))};
+  return __builtin_bit_cast(bf16x8_t, w);
+}
+
 // x without the bits of it under `mask`, exactly.
 __device__ __forceinline__ float rest_of(float x, uint32_t mask) {
   return x - __uint_as_float(__float_as_uint(x) & mask);
@@ -321,8 +346,7 @@ __device__ __forceinline__ float sum_columns(float x) {
 
 // Fold a unit into the state.
 template <int kCols>
-__device__ __forceinline__ void fold_unit(const Unit& u, const Mask& mask, const Query<kCols>& q,
-                                          float scale, int c, State& st) {
+__device__ __forceinline__ void fold_unit(const Unit& u, const Mask& mask, const Query& q, float scale, int c, State& st) {
   constexpr uint32_t kLow16 = 0x05040100u, kHigh16 = 0x07060302u;
   // Scale bytes to exponent fields; the bits around them do not count.
   float vs[8];
@@ -348,21 +372,27 @@ __device__ __forceinline__ void fold_unit(const Unit& u, const Mask& mask, const
       odd[e] = __builtin_amdgcn_perm(d[2 * e + 1], d[2 * e], kHigh16);
     }
   };
+  const uint32_t ks[2] = {select_bits(mask.ks[0], u.ks[0], 1u),
+                          select_bits(mask.ks[1], u.ks[1], 1u)};
+  f32x4_t d[2];
+  if (__builtin_amdgcn_ballot_w64(min(ks[0] - 253u, ks[1] - 253u) < 2u)) {  // 253 or 254
+    far_scores(q, u.k, ks, mask.bias, d);
+  } else {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const uint32_t codes[4] = {u.k[h].x, u.k[h].y, u.k[h].z, u.k[h].w};
+      const float by = __uint_as_float(ks[h] << 23);
+      d[h] = mask.bias[h];
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        d[h] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(widen8(codes[i], by), q.part[i], d[h], 0, 0,
+                                                       0);
+    }
+  }
   float s[8];
 #pragma unroll
-  for (int h = 0; h < 2; ++h) {
-    const i32x8_t k = {(int)u.k[h].x, (int)u.k[h].y, (int)u.k[h].z, (int)u.k[h].w, 0, 0, 0, 0};
-    const int ks = (int)select_bits(mask.ks[h], u.ks[h], 127u);
-    f32x4_t d = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(k, q.part[0], mask.bias[h], 4, 0, 0,
-                                                                 ks, 0, q.scale[0]);
-    if constexpr (kCols == 16)
-      d = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(k, q.part[1], d, 4, 0, 0, ks, 0,
-                                                           q.scale[1]);
-#pragma unroll
-    for (int e = 0; e < 4; ++e)
-      // Columns c and c +- kCols hold the two parts: a rotation within the row.
-      s[4 * h + e] = kCols == 16 ? d[e] : d[e] + dpp_f32<0x120 + kCols % 16>(d[e]);
-  }
+  for (int e = 0; e < 8; ++e) s[e] = d[e >> 2][e & 3];
+  __builtin_amdgcn_s_setprio(1);  // (measured: 2-3 % of a long batch)
   float mx = s[0];
 #pragma unroll
   for (int e = 1; e < 8; ++e) mx = fmaxf(mx, s[e]);
@@ -425,6 +455,7 @@ __device__ __forceinline__ void fold_unit(const Unit& u, const Mask& mask, const
   two_dims(std::integral_constant<int, 1>{});
   two_dims(std::integral_constant<int, 2>{});
   two_dims(std::integral_constant<int, 3>{});
+  __builtin_amdgcn_s_setprio(0);
 }
 
 // The q-heads of segment (b, hc): h0 .. h0 + the result - 1.
@@ -651,7 +682,7 @@ __global__ __launch_bounds__(kThreads, 2) void kv_decode_kernel(DecodeArgs a) {
         ends = wave == min(at.units, kWaves) - 1;
       }
       const int row = at.b * a.Hq + h0, heads = nh;
-      const Query<kCols> q = split_query<kCols>(raw, a.flip, c);
+      const Query q = query_operands(raw, a.flip);
       at.left -= (uint32_t)k;
       if (at.left > 0) {  // the next segment's queries are on their way meanwhile
         next_segment(a, at);

@@ -39,6 +39,22 @@ def check_exact(got, want, mass, tol=TOL):
     assert not bad.any(), f"{bad.sum()} of {bad.size}"
 
 
+def most_difference(q, cache, table, lens):
+    G = q.shape[1] // cache.shape[1]
+    most = 0.0
+    for b, n in enumerate(lens):
+        for h in range(q.shape[1]):
+            s = ref.mxfp4_rows(cache, table[b], n, h // G)[0] @ q[b, h]
+            most = max(most, s.max() - s.min())
+    return most
+
+
+def fitting(q, cache, table, lens):
+    """A power of two as scale."""
+    return 2.0 ** math.floor(math.log2(A / (most_difference(q, cache, table, lens)
+                                            * math.log2(math.e))))
+
+
 def exact_inputs(seed, B, Hq, Hkv, bs=16):
     """Requests of 2 to 4 tokens: (q [B, Hq, 128] float64, cache, table, lengths, scale)."""
     rng = np.random.default_rng(seed)
@@ -50,13 +66,7 @@ def exact_inputs(seed, B, Hq, Hkv, bs=16):
     table = np.arange(B)[:, None].astype(np.int32)
     # Scores: multiples of 0.25 below 128 * 8 * 12; their differences times scale and
     # log2(e) below A.
-    most = 0.0
-    for b, n in enumerate(lens):
-        for h in range(Hq):
-            s = ref.mxfp4_rows(cache, table[b], n, h // (Hq // Hkv))[0] @ q[b, h]
-            most = max(most, s.max() - s.min())
-    scale = 2.0 ** math.floor(math.log2(A / (most * math.log2(math.e))))
-    return q, cache, table, lens, scale
+    return q, cache, table, lens, fitting(q, cache, table, lens)
 
 
 def model(q, cache, table, lens, scale, parts, heads_per_kv):
@@ -152,3 +162,71 @@ def test_ordinary_batches(gpu, Hq, Hkv):
     want, _, _, _ = ref.mxfp4_attention(q, cache, table, lens, scale)
     for how in ({}, {"num_workgroups": 37}):
         assert off(run(gpu, q, cache, table, lens, scale, **how), want) < NORM
+
+
+def silence(cache, dims):
+    """Keys of all tokens zero in these dims (of either sign)."""
+    for r in range(16):
+        for d in dims:
+            at = ref.tile_offsets(r, d)[0]
+            cache[..., at] &= 0xF7 if d % 2 == 0 else 0x7F
+            cache[..., at] &= 0xF8 if d % 2 == 0 else 0x8F
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("loud", [2.0 ** 8, 2.0 ** 12, 2.0 ** 30, 2.0 ** 100])
+@pytest.mark.parametrize("Hq,Hkv", GROUPS)
+def test_quiet_dims_beside_loud_ones(gpu, Hq, Hkv, loud):
+    """Queries with a few dims many times the others, which keys that are zero there take out of
+    the score: what the other dims say is not lost."""
+    q, cache, table, lens, _ = exact_inputs(Hq, 24, Hq, Hkv)
+    dims = [3, 40, 41, 127]
+    silence(cache, dims)
+    rng = np.random.default_rng(1)
+    q[..., dims] = rng.integers(4, 9, q[..., dims].shape) * loud
+    q[::3, ::2, dims] = 1.0  # and heads without, beside them
+    scale = 2.0 ** -9
+    want, mass, _, _ = ref.mxfp4_attention(q, cache, table, lens, scale)
+    assert most_difference(q, cache, table, lens) * scale * math.log2(math.e) <= A
+    check_exact(run(gpu, q, cache, table, lens, scale), want, mass)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("loud", [2.0 ** 8, 2.0 ** 10])
+@pytest.mark.parametrize("Hq,Hkv", GROUPS)
+def test_sums_of_loud_and_quiet_dims(gpu, Hq, Hkv, loud):
+    """The same with keys that are not zero there: the sum has all its terms. (4 terms of up to
+    8 * 12 * 2^10 and 124 of up to 96, in steps of 0.25: 21 bits.)"""
+    q, cache, table, lens, _ = exact_inputs(Hq, 24, Hq, Hkv)
+    dims = [3, 40, 41, 127]
+    rng = np.random.default_rng(1)
+    q[..., dims] = rng.integers(4, 9, q[..., dims].shape) * loud
+    scale = fitting(q, cache, table, lens)
+    want, mass, _, _ = ref.mxfp4_attention(q, cache, table, lens, scale)
+    check_exact(run(gpu, q, cache, table, lens, scale), want, mass)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("keys,at", [((0, 4), 124), ((4, 7), 122), ((100, 103), 26),
+                                     ((246, 250), -121),
+                                     ((252, 255), -126)])
+@pytest.mark.parametrize("tiny", [False, True])
+@pytest.mark.parametrize("Hq,Hkv", [(4, 1), (8, 1), (16, 1)])
+def test_far_scales(gpu, Hq, Hkv, keys, at, tiny):
+    """Keys of very small and very large scales under queries of the opposite size; slots behind
+    the last token hold anything. With `tiny`, an element far below its head's largest too."""
+    rng = np.random.default_rng(2)
+    q, cache, table, lens, _ = exact_inputs(Hq, 24, Hq, Hkv)
+    cache[..., 2048:2112] = rng.integers(*keys, cache[..., 2048:2112].shape)
+    for b, n in enumerate(lens):
+        for r in range(n, 16):
+            cache[b, :, 0, [2048 + g * 16 + r for g in range(4)]] = rng.integers(0, 256, (4, Hkv))
+            cache[b, :, 0, [2112 + r // 4 * 16 + g * 4 + r % 4 for g in range(4)]] = 255
+    q *= 2.0 ** at
+    if tiny:
+        silence(cache, [64])
+        q[..., 64] = 2.0 ** -133
+    scale = 2.0 ** -10
+    assert most_difference(q, cache, table, lens) * scale * math.log2(math.e) <= A
+    want, mass, _, _ = ref.mxfp4_attention(q, cache, table, lens, scale)
+    check_exact(run(gpu, q, cache, table, lens, scale), want, mass)
