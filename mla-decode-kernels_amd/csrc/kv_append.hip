@@ -101,17 +101,37 @@ __device__ __forceinline__ void others(const F (&x)[8], F (&y)[8], const Turn& t
   }
 }
 
+// The mean of the squares of a row of 8 kLanes dims, kLanes lanes each, plus eps.
+template <int kLanes>
+__device__ __forceinline__ float mean_square(const float (&x)[8], float eps) {
+  float ss = 0.f;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) ss = fmaf(x[e], x[e], ss);
+  return (kLanes == 16 ? row16_sum(ss) : gqa::wave_sum(ss)) * (1.f / (8 * kLanes)) + eps;
+}
+
+// x / sqrt(mean(x^2) + eps) * w. Squares can leave fp32's range on either side (values
+// past 1e19, or tiny ones with next to no eps): such a row is taken again times a
+// power of two. (Up: eps is below 2^-100 there, so times 2^200 it still fits.)
+template <int kLanes>
+__device__ __forceinline__ void norm_row(float (&x)[8], const float (&w)[8], float eps) {
+  float v = mean_square<kLanes>(x, eps);
+  const bool ordinary = v >= 0x1p-100f && v < __builtin_inff();
+  if (__builtin_amdgcn_ballot_w64(!ordinary)) {
+    const float f = ordinary ? 1.f : v < 1.f ? 0x1p100f : 0x1p-68f;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) x[e] *= f;
+    v = mean_square<kLanes>(x, eps * f * f);
+  }
+  const float r = rsqrtf(v);
+#pragma unroll
+  for (int e = 0; e < 8; ++e) x[e] = x[e] * r * w[e];
+}
+
 // Norm over the head's 128 dims (16 lanes), then the rotation.
 __device__ __forceinline__ void norm_turn(float (&x)[8], bool norm, const float (&w)[8], float eps,
                                           const Turn& t, bool rotate, Pairs pairs) {
-  if (norm) {
-    float ss = 0.f;
-#pragma unroll
-    for (int e = 0; e < 8; ++e) ss = fmaf(x[e], x[e], ss);
-    const float r = rsqrtf(row16_sum(ss) * (1.f / kDim) + eps);
-#pragma unroll
-    for (int e = 0; e < 8; ++e) x[e] = x[e] * r * w[e];
-  }
+  if (norm) norm_row<16>(x, w, eps);
   if (!rotate) return;
   float y[8];
   others(x, y, t, pairs);
@@ -384,14 +404,9 @@ __global__ __launch_bounds__(64 * kWaves) void kv_append_mla_kernel(kv_append_ml
     unpack8(raw[j], x);
     if (pass0 + j == 0) {
       if (a.c_weight) {
-        float ss = 0.f;
-#pragma unroll
-        for (int e = 0; e < 8; ++e) ss = fmaf(x[e], x[e], ss);
-        const float r = rsqrtf(gqa::wave_sum(ss) * (1.f / kLatent) + a.eps);
         float w[8];
         load_weights(a.c_weight, a.c_weight_type, 8 * lane, w);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) x[e] = x[e] * r * w[e];
+        norm_row<64>(x, w, a.eps);
         raw[j] = pack8(x);
       }
       if (block >= 0) *reinterpret_cast<uint4*>(dst + 8 * lane) = raw[j];
