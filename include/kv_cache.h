@@ -99,7 +99,7 @@ typedef struct kv_append_args {
   uint16_t* k_cache;
   uint16_t* v_cache;
   uint8_t* mxfp4_cache;
-  const int* block_table;
+  const int* block_table; /* may be null with B = 0, as may seq_lens */
   const int* seq_lens;
   const int* cu_seqlens;     /* null: one token a request */
   const int* rope_positions; /* [T], null: the tokens' positions */

@@ -433,6 +433,12 @@ bool bad_weight(const void* w, int type) {
 
 bool misaligned(const void* p, uintptr_t to) { return (reinterpret_cast<uintptr_t>(p) & (to - 1)) != 0; }
 
+// (Without requests the index tensors are empty and may have no memory; the kernels
+// read neither then.)
+bool no_index(int B, const int* block_table, const int* seq_lens) {
+  return B > 0 && (!block_table || !seq_lens);
+}
+
 // Sizes that every append and read shares.
 hipError_t check_sizes(int T, int B, bool ragged, int num_blocks, int block_size, int max_blocks) {
   if (T < 0 || T > KV_MAX_TOKENS || B < 0 || num_blocks < 0) return hipErrorInvalidValue;
@@ -454,7 +460,7 @@ hipError_t check_append(const kv_append_args& a, bool mx) {
   if (bad_weight(a.q_weight, a.q_weight_type) || bad_weight(a.k_weight, a.k_weight_type))
     return hipErrorInvalidValue;
   if (a.T == 0) return hipSuccess;
-  if (!a.q || !a.k || !a.v || !a.q_out || !a.block_table || !a.seq_lens)
+  if (!a.q || !a.k || !a.v || !a.q_out || no_index(a.B, a.block_table, a.seq_lens))
     return hipErrorInvalidValue;
   if (a.num_blocks > 0) {
     if (mx ? (!a.mxfp4_cache || misaligned(a.mxfp4_cache, 4))
@@ -509,7 +515,7 @@ extern "C" int kv_read_mxfp4_launch(const uint8_t* mxfp4_cache, const int* block
   if (e != hipSuccess) return e;
   if (Hkv < 1 || Hkv > 4096 || block_size % kTileTokens != 0) return hipErrorInvalidValue;
   if (T == 0) return hipSuccess;
-  if (!block_table || !seq_lens || !k_out || !v_out || misaligned(k_out, 16) ||
+  if (no_index(B, block_table, seq_lens) || !k_out || !v_out || misaligned(k_out, 16) ||
       misaligned(v_out, 16) || (num_blocks > 0 && (!mxfp4_cache || misaligned(mxfp4_cache, 4))))
     return hipErrorInvalidValue;
   kv_read_mxfp4_kernel<<<dim3((unsigned)((T + 3) / 4), (Hkv + kWaves - 1) / kWaves), 64 * kWaves, 0,
@@ -528,7 +534,8 @@ extern "C" int kv_append_mla_launch(const kv_append_mla_args* args, hipStream_t 
   if (a.h_q < 1 || a.h_q > 4096 || a.table_rows < 0 || bad_weight(a.c_weight, a.c_weight_type))
     return hipErrorInvalidValue;
   if (a.T == 0) return hipSuccess;
-  if (!a.q_pe || !a.c || !a.k_pe || !a.q_out || !a.block_table || !a.seq_lens || !a.cos_sin ||
+  if (!a.q_pe || !a.c || !a.k_pe || !a.q_out || no_index(a.B, a.block_table, a.seq_lens) ||
+      !a.cos_sin ||
       (a.num_blocks > 0 && (!a.kv_cache || misaligned(a.kv_cache, 16))))
     return hipErrorInvalidValue;
   const int passes = 1 + (a.h_q + 8) / 8;  // the latent row, then h_q + 1 rotary rows

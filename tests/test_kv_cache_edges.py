@@ -76,3 +76,30 @@ def test_mla_norm_of_very_large_and_small_rows(gpu, eps):
                         c_weight=w.to(gpu), eps=eps)
     want = ref.norm(f64(c), w.numpy(), float(np.float32(eps)))
     check_rows(cache.view(-1, 576)[:T, :512], want, np.abs(want))
+
+
+def step(gpu, T, Hq=8, Hkv=2):
+    gen = torch.Generator().manual_seed(T)
+    return [torch.randn(T, h, D, generator=gen).bfloat16().to(gpu) for h in (Hq, Hkv, Hkv)]
+
+
+def test_rows_without_any_request(gpu):
+    """No request (index tensors made empty, without memory) but rows: all of them padding."""
+    q, k, v = step(gpu, 5)
+    table = torch.empty(0, 3, dtype=torch.int32, device=gpu)
+    lens = torch.empty(0, dtype=torch.int32, device=gpu)
+    cu = torch.zeros(1, dtype=torch.int32, device=gpu)
+    assert table.data_ptr() == 0 and lens.data_ptr() == 0
+    kc, vc = (torch.ones(3, 16, 2, D, dtype=torch.bfloat16, device=gpu) for _ in range(2))
+    mx = torch.ones(3, 2, 1, 2176, dtype=torch.uint8, device=gpu)
+    mla = torch.ones(3, 16, 1, 576, dtype=torch.bfloat16, device=gpu)
+    cs, cs64 = kv_cache.rotary_table(4, 128), kv_cache.rotary_table(4, 64)
+    outs = [kv_cache.kv_append(q, k, v, kc, vc, table, lens, cs, cu),
+            kv_cache.kv_append_mxfp4(q, k, v, mx, table, lens, cs, cu),
+            kv_cache.mla_append(q[..., :64], q.view(5, -1)[:, :512], k[:, 0, :64], mla, table, lens,
+                                cs64, cu),
+            *kv_cache.kv_read_mxfp4(mx, table, lens, cu, 5)]
+    for out in outs:
+        assert out.shape[0] == 5 and not out.any()
+    for cache in (kc, vc, mx, mla):
+        assert (cache == 1).all()
