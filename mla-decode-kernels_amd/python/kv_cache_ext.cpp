@@ -72,6 +72,12 @@ Rows rows_of(const char* name, const Tensor& t) {
           heads ? t.size(1) : 1, t.stride(0), heads ? t.stride(1) : 0, t.size(-1)};
 }
 
+// The stride of a dimension that two arrays share, -1 if they differ. (Of a dimension
+// of size 1 it can be anything and means nothing.)
+int64_t common_stride(int64_t sx, int64_t nx, int64_t sy, int64_t ny) {
+  return nx <= 1 ? sy : ny <= 1 || sx == sy ? sx : -1;
+}
+
 // Whether x and y surely have no element in common: apart as a whole, or, with
 // the same token (and head) stride, in every period of it (two views of one
 // projection's output).
@@ -84,9 +90,11 @@ bool disjoint(const Rows& x, const Rows& y) {
     return wx <= m && m + wy <= period;
   };
   const int64_t d = y.base - x.base;
-  if (x.st == y.st && apart(d, x.st, x.token_width(), y.token_width())) return true;
-  return x.st == y.st && x.sh == y.sh && x.sh > 0 && x.st % x.sh == 0 &&
-         apart(d, x.sh, x.width, y.width);
+  const int64_t st = common_stride(x.st, x.T, y.st, y.T);
+  const int64_t sh = common_stride(x.sh, x.heads, y.sh, y.heads);
+  if (apart(d, st, x.token_width(), y.token_width())) return true;
+  const bool one_token = x.T == 1 && y.T == 1;
+  return st >= 0 && sh > 0 && (one_token || st % sh == 0) && apart(d, sh, x.width, y.width);
 }
 
 void check_no_overlap(const Rows& x, const Rows& y) {
@@ -193,7 +201,8 @@ Tensor output_for(const Tensor& q, const OptTensor& q_out, const char* shape) {
 
 void check_output(const Rows& q, const Rows& out, std::initializer_list<Rows> inputs) {
   check_written(out);
-  const bool in_place = q.base == out.base && q.st == out.st && q.sh == out.sh;
+  const bool in_place = q.base == out.base && (q.T <= 1 || q.st == out.st) &&
+                        (q.heads <= 1 || q.sh == out.sh);
   if (!in_place) check_no_overlap(q, out);
   for (const Rows& r : inputs) check_no_overlap(r, out);
 }

@@ -103,3 +103,36 @@ def test_rows_without_any_request(gpu):
         assert out.shape[0] == 5 and not out.any()
     for cache in (kc, vc, mx, mla):
         assert (cache == 1).all()
+
+
+def test_strides_of_single_tokens_and_heads_do_not_matter(gpu):
+    """q itself as q_out through another view of the same rows: a dimension of size 1 may have any
+    stride."""
+    table = torch.zeros(1, 1, dtype=torch.int32, device=gpu)
+    one = torch.ones(1, dtype=torch.int32, device=gpu)
+    cs, cs64 = kv_cache.rotary_table(4, 128), kv_cache.rotary_table(4, 64)
+    kc, vc = (torch.zeros(1, 16, 2, D, dtype=torch.bfloat16, device=gpu) for _ in range(2))
+    q, k, v = step(gpu, 1)
+    want = kv_cache.kv_append(q, k, v, kc, vc, table, one, cs)
+    qkv = torch.cat([q, k, v], dim=1)
+    view = qkv[:, :8]
+    same = view.as_strided((1, 8, D), (8 * D, D, 1))
+    assert view.stride() != same.stride()
+    kv_cache.kv_append(view, qkv[:, 8:10], qkv[:, 10:], kc, vc, table, one, cs, q_out=same)
+    assert torch.equal(view, want) and torch.equal(qkv[:, 8:10], k)
+    # One head: its stride may be anything as well.
+    T = 3
+    tables = torch.arange(T, dtype=torch.int32, device=gpu)[:, None]
+    lens = torch.ones(T, dtype=torch.int32, device=gpu)
+    row = torch.randn(T, 640, generator=torch.Generator().manual_seed(0)).bfloat16().to(gpu)
+    cache = torch.zeros(T, 16, 1, 576, dtype=torch.bfloat16, device=gpu)
+    q1 = row[:, 576:].as_strided((T, 1, 64), (640, 64, 1), 576)
+    q2 = row[:, 576:].as_strided((T, 1, 64), (640, 1, 1), 576)
+    args = (row[:, :512], row[:, 512:576], cache, tables, lens, cs64)
+    want = kv_cache.mla_append(q1, *args)
+    kv_cache.mla_append(q1, *args, q_out=q2)
+    assert torch.equal(q1, want)
+    # Rows that do overlap are still refused.
+    with pytest.raises(RuntimeError, match="overlap"):
+        kv_cache.kv_append(view, k, v, kc, vc, table, one, cs,
+                           q_out=qkv.as_strided((1, 8, D), (8 * D, D, 1), D))
