@@ -230,3 +230,21 @@ def test_far_scales(gpu, Hq, Hkv, keys, at, tiny):
     assert most_difference(q, cache, table, lens) * scale * math.log2(math.e) <= A
     want, mass, _, _ = ref.mxfp4_attention(q, cache, table, lens, scale)
     check_exact(run(gpu, q, cache, table, lens, scale), want, mass)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("Hq", [1, 8, 16])
+@pytest.mark.parametrize("lens", [[131072], [40, 70000], [70000, 3, 66000, 1]])
+def test_segments_cut_into_many_pieces(gpu, lens, Hq):
+    """One kv-head, so that a request spans more workgroups than the merge's waves have lanes; in
+    front of it, short ones that start in the middle of a share."""
+    bs = 256
+    q, cache, table, scale = ordinary_inputs(Hq, lens, Hq, 1, bs)
+    # Shares of 16 units (of 32 tokens) at least: the longest takes that many workgroups.
+    units = [-(-n // 32) for n in lens]
+    assert max(units) / (sum(units) / min(256, -(-sum(units) // 16))) > 65
+    want, _, _, _ = ref.mxfp4_attention(q, cache, table, lens, scale)
+    got = run(gpu, q, cache, table, lens, scale, num_workgroups=256)
+    assert off(got, want) < NORM
+    assert np.array_equal(got, run(gpu, q, cache, table, lens, scale, num_workgroups=256))
+    assert off(run(gpu, q, cache, table, lens, scale), want) < NORM
