@@ -375,7 +375,8 @@ __device__ __forceinline__ void fold_unit(const Unit& u, const Mask& mask, const
   const uint32_t ks[2] = {select_bits(mask.ks[0], u.ks[0], 1u),
                           select_bits(mask.ks[1], u.ks[1], 1u)};
   f32x4_t d[2];
-  if (__builtin_amdgcn_ballot_w64(min(ks[0] - 253u, ks[1] - 253u) < 2u)) {  // 253 or 254
+  // (255 as well: one NaN key makes all of the unit's heads NaN.)
+  if (__builtin_amdgcn_ballot_w64(max(ks[0], ks[1]) >= 253u)) {
     far_scores(q, u.k, ks, mask.bias, d);
   } else {
 #pragma unroll
