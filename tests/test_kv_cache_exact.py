@@ -25,7 +25,13 @@ from oracle import kv_reference as ref
 
 D = 128
 A = 4.0
-TOL = (2 * (1.5 * A * math.log(2) + 1) + 2 * 14 + 2) * 2.0 ** -23
+
+
+def tolerance(a):
+    return (2 * (1.5 * a * math.log(2) + 1) + 2 * 14 + 2) * 2.0 ** -23
+
+
+TOL = tolerance(A)
 
 
 def half_step(x):
@@ -33,8 +39,8 @@ def half_step(x):
     return 2.0 ** (np.floor(np.log2(np.maximum(np.abs(x), 2.0 ** -126))) - 8)
 
 
-def check_exact(got, want, mass, tol=TOL):
-    over = tol * mass
+def check_exact(got, want, mass, tol=TOL, under=0.0):
+    over = tol * mass + under
     bad = ~(np.abs(got - want) <= half_step(np.abs(want) + over) + over)
     assert not bad.any(), f"{bad.sum()} of {bad.size}"
 
@@ -101,8 +107,12 @@ def test_the_check_tells_weights_of_fewer_bits():
 
 
 def run(gpu, q, cache, table, lens, scale, **how):
+    assert np.array_equal(torch.from_numpy(q).bfloat16().double().numpy(), q)
+    return run_any(gpu, q, cache, table, lens, scale, **how)
+
+
+def run_any(gpu, q, cache, table, lens, scale, **how):
     qt = torch.from_numpy(q).bfloat16()
-    assert np.array_equal(qt.double().numpy(), q)
     index = lambda x: torch.as_tensor(np.asarray(x), dtype=torch.int32).to(gpu)  # noqa: E731
     out = kv_cache.gqa_decode_mxfp4(qt.to(gpu), torch.from_numpy(cache).to(gpu), index(table),
                                     index(lens), scale, **how)
@@ -174,6 +184,21 @@ def silence(cache, dims):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("times", [0.0, -1.0, 16.0, -64.0, 1024.0])
+@pytest.mark.parametrize("Hq,Hkv", [(4, 1), (8, 1), (16, 1)])
+def test_exact_scores_under_other_scales(gpu, Hq, Hkv, times):
+    """No softmax at all, the smallest score first, one key taking nearly all. There a weight,
+    relative to the largest one, can lie below fp32's smallest normal number, 2^-126, and count as
+    0, and so can its second and third part and their products: 4 * 2^-126 of the largest |value|
+    for each of up to 4 keys (all that is left where the largest weight's value is 0)."""
+    q, cache, table, lens, scale = exact_inputs(Hq, 48, Hq, Hkv)
+    want, mass, _, _ = ref.mxfp4_attention(q, cache, table, lens, scale * times)
+    largest = 6.0 * 2.0 ** (cache[..., 2112:].max() - 127.0)
+    check_exact(run(gpu, q, cache, table, lens, scale * times), want, mass,
+                tolerance(A * max(abs(times), 1.0)), 4 * 4 * 2.0 ** -126 * largest)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("loud", [2.0 ** 8, 2.0 ** 12, 2.0 ** 30, 2.0 ** 100])
 @pytest.mark.parametrize("Hq,Hkv", GROUPS)
 def test_quiet_dims_beside_loud_ones(gpu, Hq, Hkv, loud):
@@ -230,6 +255,25 @@ def test_far_scales(gpu, Hq, Hkv, keys, at, tiny):
     assert most_difference(q, cache, table, lens) * scale * math.log2(math.e) <= A
     want, mass, _, _ = ref.mxfp4_attention(q, cache, table, lens, scale)
     check_exact(run(gpu, q, cache, table, lens, scale), want, mass)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("keys,at", [((126, 129), 0), ((252, 255), -126)])
+@pytest.mark.parametrize("Hq,Hkv", [(4, 1), (8, 1), (16, 1)])
+def test_queries_that_are_not_finite(gpu, Hq, Hkv, keys, at):
+    """NaN for the head of an infinity or NaN, whatever the keys' scales and signs; for no other."""
+    rng = np.random.default_rng(4)
+    q, cache, table, lens, _ = exact_inputs(Hq, 24, Hq, Hkv)
+    cache[..., 2048:2112] = rng.integers(*keys, cache[..., 2048:2112].shape)
+    cache[5:, ..., :1024] = 0x33  # keys of one sign: scores of one infinity
+    q *= 2.0 ** at
+    bad = np.zeros(q.shape[:2], dtype=bool)
+    for b, h, d, x in ((0, 1, 77, np.nan), (3, 0, 3, np.inf), (7, Hq - 1, 127, -np.inf),
+                       (8, 2, 31, np.inf)):
+        q[b, h, d], bad[b, h] = x, True
+    got = torch.from_numpy(run_any(gpu, q, cache, table, lens, 2.0 ** -10))
+    assert torch.isnan(got[torch.from_numpy(bad)]).all()
+    assert torch.isfinite(got[torch.from_numpy(~bad)]).all()
 
 
 @pytest.mark.gpu
