@@ -34,13 +34,14 @@
  * batch). Padding writes nothing to a cache, and its row of q_out or of the
  * rows read back is zeros. Rows whose position is past the block table, or
  * whose block id is outside [0, num_blocks), write nothing to the cache either
- * (and read back as zeros); their q_out row is computed. Requests of one call
- * must not share a block that the call writes.
+ * (and read back as zeros); their q_out row is computed. A block that a call
+ * writes stands once in the call's table rows: no two of its requests share it,
+ * and none lists it twice.
  *
  * Launchers are asynchronous on `stream`, allocate nothing, keep nothing
  * between calls, may be captured into graphs, and return 0 or a hipError_t
  * code (hipErrorInvalidValue for arguments rejected before any launch). They
- * run on the current device. Results are bitwise deterministic. No reference
+ * run on the current device. The same call gives the same bits. No reference
  * counterpart: the reference's benches fill their caches with torch.
  */
 #ifndef KV_CACHE_H_
@@ -121,7 +122,8 @@ GQA_DECODE_API int kv_append_launch(const kv_append_args* args, hipStream_t stre
  * its largest magnitude into (3.5, 7] (at least 2^-126), an element's code the
  * nearest one, ties to the even code; a group that holds an infinity or NaN
  * gets scale 255. Keys are normed and turned in fp64, so the codes are those of
- * the formula, whichever launch wrote them. */
+ * the formula, whichever launch wrote them (what is past fp32's range by then
+ * counts as its largest value). */
 GQA_DECODE_API int kv_append_mxfp4_launch(const kv_append_args* args, hipStream_t stream);
 
 /* The keys and values of the rows that an append with the same T, cu_seqlens,
@@ -176,11 +178,19 @@ GQA_DECODE_API int kv_append_mla_launch(const kv_append_mla_args* args, hipStrea
  * B * ceil(max_blocks * block_size / 32) * Hkv * ceil(Hq / Hkv / 16) is at most
  * 2^31 - 1, and so are the bytes of a block (of all heads).
  *
- * Token-balanced: a grid of num_workgroups workgroups (<= 0: chosen from the
- * sizes and the current device), each taking an equal share of the batch's
- * 32-token units, whatever the lengths; a second launch merges the requests
- * cut at share boundaries, in share order, so results are bitwise reproducible
- * for given lengths and num_workgroups. The host never reads seq_lens.
+ * num_workgroups > 0: token-balanced. Each workgroup of that grid takes an equal
+ * share of the batch's 32-token units, whatever the lengths, and a second launch
+ * merges the segments (a request's tokens for up to 16 q-heads of one kv-head)
+ * cut at share boundaries, in share order: the bits of a result are those of the
+ * lengths, the batch and num_workgroups.
+ * num_workgroups <= 0: chosen from the sizes and the current device. Tables of up
+ * to 64 units a request (48 where segments are fewer than a quarter of the CUs) keep
+ * segments whole, in one launch: a workgroup to each segment if they are no more
+ * than the CUs, else shares whose ends are moved to the next segment's start. Wider
+ * tables take the token-balanced launch with a workgroup to each CU. The choice, and
+ * with it the order of the sums, depends on max_blocks * block_size, not on the
+ * lengths: the host never reads seq_lens. Where short requests lie behind a wide
+ * table, a max_blocks (and table) cut to the longest saves 1-5 us.
  * workspace: kv_decode_mxfp4_workspace_bytes(B, Hq, Hkv, block_size,
  * max_blocks, num_workgroups) bytes (it may be 0), 16-byte aligned,
  * uninitialised; launches that share one must not overlap. */

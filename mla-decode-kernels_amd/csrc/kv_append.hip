@@ -3,14 +3,14 @@
 // the step's rows; and the read-back of rows of the 4-bit cache.
 //
 // What bounds them is the bytes, read once and written once, once there are enough
-// of them: 7255 tokens (32Q/8KV, half of each head turned) 180 MB in 35 us of GPU time,
-// 5.1 TB/s, the rate of a plain copy; below some 500 tokens the chain of latencies
+// of them: 7255 tokens (32Q/8KV, half of each head turned) 180 MB in 35.8 us of GPU
+// time, 5.0 TB/s, a plain copy of as many 5.1; below some 500 tokens the chain of latencies
 // (request, length, block id, angles), 3-5 us. A wave takes four tokens, 16
 // lanes (a DPP row) each, 8 dims a lane, and walks heads: the tokens' places
 // and their angles (16 registers) are found once and serve every head. In
 // the 4-bit cache four tokens of a request, if they are aligned, are one whole
-// 256-byte line of value codes. The 4-bit append of 3880 tokens with norms moves 81 MB
-// in 23 us (3.5 TB/s): fp64 costs 2 us of them, the norms 2, the search for places 1.
+// 256-byte line of value codes. The 4-bit append of 3880 tokens with norms moves 86 MB
+// in 23 us (3.7 TB/s): fp64 costs 2 us of them, the norms 2, the search for places 1.
 #include <type_traits>
 
 #include "kv_cache.h"
@@ -223,9 +223,9 @@ __device__ __forceinline__ void store_mx(const kv_append_args& a, int block, int
 
 // Heads a wave takes: R of the queries, of the values, and of the keys of the
 // bf16 cache; one of the keys of the 4-bit cache, whose fp64 arithmetic on
-// several rows at once would take the registers of half the waves (append and
-// read-back of 3880 tokens: 37 us at 4 keys a wave, 32 us at 1; taken one after the
-// other in a loop 32.9 at 4 and 29.5 at 2, to 29.3).
+// several rows at once would take the registers of half the waves. (Append and
+// read-back of 3880 tokens: 29.3 us; with the keys one after the other in a loop 29.5 at
+// 2 a wave and 32.9 at 4.)
 template <bool kMx, int R>
 struct Tasks {
   static constexpr int kKeys = kMx ? 1 : R;

@@ -38,8 +38,8 @@
 // workspace, where a second kernel folds them in order.
 //
 // What bounds it: HBM, at 136 bytes a token and kv-head. 32 requests of 8192 tokens
-// (32Q/8KV, blocks of 16: 286 MB) take 49.3 us, merge launch and all (5.8 TB/s); 64
-// ragged ones up to 32768 (64Q/8KV, blocks of 64: 1047 MB) 180 us (5.8 TB/s). The same
+// (32Q/8KV, blocks of 16: 286 MB) take 48.4 us, merge launch and all (5.9 TB/s); 64
+// ragged ones up to 32768 (64Q/8KV, blocks of 64: 1047 MB) 178 us (5.9 TB/s). The same
 // launches with the loads alone and no arithmetic took 47 and 164 us. 8 waves a
 // workgroup and one workgroup a CU, two waves a SIMD, with one unit (4352 bytes a
 // wave) in flight behind the one that is folded: two units ahead 2-10 % slower, 4
@@ -858,12 +858,12 @@ struct Shape {
 
 // Short sequences keep their segments whole: one launch, no merge, for shares
 // that are even only to a segment. Measured on MI355X, 32Q/8KV, block 16, whole
-// against balanced: tables of 1000 tokens, 1 to 64 full requests 9.1-17.4 us
-// against 10.8-18.1, 8 to 256 of U[1, 1000] 9.1-42.0 against 13.0-44.1; of 2000
-// tokens 8, 32 and 64 full requests 13.1, 15.4 and 28.8 against 13.0, 18.0 and
-// 28.9, 8 to 256 ragged ones 10.2-60.7 against 12.3-64.1, but a single request
-// (8 segments) 12.7 against 11.6 (at 1500 tokens 10.8 against 11.4); of 4000
-// tokens 1 and 8 full requests 20.0 and 20.8 against 11.7 and 15.6.
+// against balanced: tables of 1000 tokens, 1 to 64 full requests 9.4-18.5 us
+// against 10.8-19.9, 8 to 256 of U[1, 1000] 9.6-45.9 against 13.4-46.8; of 2000
+// tokens 8, 32 and 64 full requests 13.8, 16.3 and 29.4 against 13.1, 19.2 and
+// 29.4, 8 to 256 ragged ones 10.7-63.5 against 12.5-66.6, but a single request
+// (8 segments) 13.4 against 12.2 (at 1500 tokens 11.5 against 11.9); of 4000
+// tokens 1 and 8 full requests 21.0 and 21.7 against 12.2 and 16.4.
 constexpr int kWholeUnits = 64, kFewWholeUnits = 48;
 bool keep_whole(int64_t units, int64_t segments, int cus) {
   return units <= (4 * segments >= cus ? kWholeUnits : kFewWholeUnits);

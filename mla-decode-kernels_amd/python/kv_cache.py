@@ -29,8 +29,8 @@ them at position seq_lens[b] - 1. A row without a place -- at or past
 cu_seqlens[B], or of a request with seq_lens[b] below its number of rows, as 0
 for an unused entry of a fixed-size batch -- is padding: it writes nothing to a
 cache and its row of the result is zeros. A position past the block table, or
-a block id outside the cache, writes nothing either. The requests of a call
-must not share a block that the call writes to.
+a block id outside the cache, writes nothing either. A block that the call writes
+to must stand once in its table rows: no other request's, and not twice in one.
 
 Norm and rotation. q_weight / k_weight (bf16 or fp32 [128]) ask for
 x / sqrt(mean(x^2) + eps) * weight over each head; cos_sin (rotary_table) turns the
@@ -89,7 +89,8 @@ kv_read_mxfp4 = _ext.kv_read_mxfp4
 mla_append = _ext.mla_append
 # gqa_decode_mxfp4(q [B, Hq, 128], kv_cache, block_table, seq_lens, scale,
 #                  num_workgroups=0) -> out [B, Hq, 128]; a request of length 0
-#   gets zeros. num_workgroups > 0 sets the token-balanced launch's grid.
+#   gets zeros. num_workgroups > 0 sets the token-balanced launch's grid; 0 chooses
+#   launch and grid from the sizes, block_table's width among them, and the device.
 gqa_decode_mxfp4 = _ext.gqa_decode_mxfp4
 
 MXFP4_TILE_TOKENS = 16
