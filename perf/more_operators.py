@@ -260,9 +260,9 @@ def _inputs(case, seed):
     if op in ("chunk8", "decode8", "append8"):
         s["cache"], s["scales"] = _filled8(pool, case, gen)
     if op == "chunk8":
-        s["whole"], s["whole_rows"] = sums(lens), sum(lens)
+        s["whole"] = sums(lens)
     if op == "append8":
-        s["back"], s["back_rows"] = sums(_tile_rows(lens, news)), sum(_tile_rows(lens, news))
+        s["back"] = sums(_tile_rows(lens, news))
         s["cos_sin"] = _angles(max(lens), case["rot"])
         s["q_weight"] = (1.0 + 0.1 * normal(D)).bfloat16() if case["norm"] else None
         s["k_weight"] = (1.0 + 0.1 * normal(D)).bfloat16() if case["norm"] else None
@@ -500,13 +500,13 @@ def run(state):
         return prefill.gqa_prefill_packed(s["q"], s["k"], s["v"], s["first"], s["first"], D ** -0.5)
     if op == "chunk8":
         k, v = kv.kv_read_fp8(s["cache"], s["scales"], s["table"], s["lens"],
-                              cu_seqlens=s["whole"], num_tokens=s["whole_rows"])
+                              cu_seqlens=s["whole"], num_tokens=sum(s["lens_list"]))
         return prefill.gqa_prefill_packed(s["q"], k, v, s["first"], s["whole"], D ** -0.5)
     q = kv.kv_append_fp8(s["q"], s["k"], s["v"], s["cache"], s["scales"], s["table"], s["lens"],
                          s["cos_sin"], cu_seqlens=s["first"], q_weight=s["q_weight"],
                          k_weight=s["k_weight"], eps=EPS, interleaved=s["case"]["interleaved"])
     k, v = kv.kv_read_fp8(s["cache"], s["scales"], s["table"], s["lens"], cu_seqlens=s["back"],
-                          num_tokens=s["back_rows"])
+                          num_tokens=sum(_tile_rows(s["lens_list"], s["news_list"])))
     return q, k, v
 
 
