@@ -403,6 +403,9 @@ struct Feed {
 // ------------------------------------------------------------------------ a wave's work
 
 constexpr float kSlack = 8.f;
+// Weights are 2^-kDown of the usual, so that sums of 2^24 weighted values of any magnitude
+// stay in fp32's range. (What is lost for it are weights below 2^-102 of the largest.)
+constexpr float kDown = 24.f;
 
 struct State {
   float m, l;        // reference of the row's weights (a raw score), their sum in this half
@@ -481,6 +484,11 @@ __device__ __forceinline__ void take_out(f32x16_t (&s)[kBlocks], int seen, uint6
   }
 }
 
+// A row's reference as weights are held against it, in units of log2.
+__device__ __forceinline__ float reference(float m, float scale) {
+  return m == kNegInf ? 0.f : fmaf(m, scale, kDown);
+}
+
 // The weights of a tile as matrix operands, rounded to bf16 (off by 2^-8 of each at most);
 // their sum is taken of what is multiplied, so that rows of equal values come out exact.
 template <int kBlocks>
@@ -507,7 +515,7 @@ __device__ __forceinline__ void soften(const f32x16_t (&s)[kBlocks], float scale
         for (int i = 0; i < 16; ++i) st.o[d][i] *= alpha;
     }
   }
-  const float ms = st.m == kNegInf ? 0.f : st.m * scale;
+  const float ms = reference(st.m, scale);
   const bf16x2_t ones = {(__bf16)1.f, (__bf16)1.f};
 #pragma unroll
   for (int b = 0; b < kBlocks; ++b)
@@ -661,7 +669,7 @@ __device__ __forceinline__ void store_row(const Args& a, int row, int split, flo
       for (int i = 0; i < 16; i += 4)
         *reinterpret_cast<f32x4_t*>(dst + 32 * d + 2 * i + 4 * h) =
             f32x4_t{o[d][i], o[d][i + 1], o[d][i + 2], o[d][i + 3]};
-    if (h == 0) a.sums[at] = make_float2(m == kNegInf ? kNegInf : m * a.scale, l);
+    if (h == 0) a.sums[at] = make_float2(m == kNegInf ? kNegInf : reference(m, a.scale), l);
     return;
   }
   const float inv = l == 0.f ? 0.f : 1.f / l;
@@ -684,7 +692,7 @@ __device__ __forceinline__ void store_row(const Args& a, int row, int split, flo
             u32x4_t{p0[0], p1[0], p0[1], p1[1]};
     }
   if (a.lse && valid && h == 0)
-    a.lse[row] = l == 0.f ? kNegInf : (m * a.scale + __log2f(l)) * gqa::kLn2;
+    a.lse[row] = l == 0.f ? kNegInf : (reference(m, a.scale) + __log2f(l)) * gqa::kLn2;
 }
 
 // The arguments that a workgroup's start needs, in registers from here on: the compiler loads
