@@ -654,6 +654,10 @@ __device__ __forceinline__ void spoil(const Spoilt& spoilt, int seen, State& st)
       if (spoilt.key[32 * d + 8 * (i / 4) + h4 + i % 4] < seen) st.o[d][i] = __builtin_nanf("");
 }
 
+// What is not finite as NaN. Finite values do not overflow, so it comes of values that are not,
+// whose tile the row sees whole: they were multiplied, and infinities may have stayed such.
+__device__ __forceinline__ float number(float x) { return fmaf(x, 0.f, x); }
+
 // A row's result: to out and lse, or to the states of split `split`.
 __device__ __forceinline__ void store_row(const Args& a, int row, int split, float m, float l,
                                           const f32x16_t (&o)[4], bool valid) {
@@ -681,8 +685,8 @@ __device__ __forceinline__ void store_row(const Args& a, int row, int split, flo
       uint32_t x[2], y[2];
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
-        x[e] = pack2(o[d][i + 2 * e] * inv, o[d][i + 2 * e + 1] * inv);
-        y[e] = pack2(o[d][i + 4 + 2 * e] * inv, o[d][i + 4 + 2 * e + 1] * inv);
+        x[e] = pack2(number(o[d][i + 2 * e] * inv), number(o[d][i + 2 * e + 1] * inv));
+        y[e] = pack2(number(o[d][i + 4 + 2 * e] * inv), number(o[d][i + 4 + 2 * e + 1] * inv));
       }
       // Half h gets all 8 dims of group i / 4 + h.
       const auto p0 = __builtin_amdgcn_permlane32_swap(x[0], y[0], false, false);
@@ -1049,7 +1053,7 @@ __global__ __launch_bounds__(64 * kMergeWaves) void prefill_merge_kernel(Args a)
   const float inv = sum == 0.f ? 0.f : 1.f / sum;
   float y[8];
 #pragma unroll
-  for (int e = 0; e < 8; ++e) y[e] = xor32_sum(gqa::xor16_sum(x[e >> 2][e & 3] * f)) * inv;
+  for (int e = 0; e < 8; ++e) y[e] = number(xor32_sum(gqa::xor16_sum(x[e >> 2][e & 3] * f)) * inv);
   if (lane < 16)
     reinterpret_cast<u32x4_t*>(a.out + (size_t)row * kDim)[i] =
         u32x4_t{pack2(y[0], y[1]), pack2(y[2], y[3]), pack2(y[4], y[5]), pack2(y[6], y[7])};

@@ -11,6 +11,8 @@ from test_prefill import D, check, f64, normal, packed_want, paged_want, pages, 
 
 pytestmark = pytest.mark.gpu
 
+INF = float("inf")
+
 def check_all(out, lse, want, label=""):
     """check, and NaN log-sum-exps in their places."""
     check(out, lse, want, label)
@@ -62,4 +64,19 @@ def test_largest_values(gpu, shape):
     want = packed_want(q, k, v, sums(news), sums(lens), 0.1, True)
     assert (np.abs(want[0]) <= most * (1 + 2.0 ** -20)).all()
     for label, got in forms(gpu, q, k, v, news, lens, 0.1):
+        check_all(*got, want, label)
+
+
+@pytest.mark.parametrize("shape", SHAPES)
+@pytest.mark.parametrize("causal", [True, False])
+def test_infinite_values(gpu, shape, causal):
+    """A value that is not finite gives NaN in its dim to every row that sees it, whether the row
+    sees its tile whole (the first keys) or in part (near the end)."""
+    q, k, v, news, lens = rows(shape, 1)
+    v[3, 0, 5], v[7, 1, 9], v[70, 0, 77] = INF, -INF, INF
+    v[71, 0, 77] = -INF
+    v[lens[0] - 2, 1, 30] = -INF
+    cu_q, cu_k = sums(news), sums(lens)
+    want = packed_want(q, k, v, cu_q, cu_k, 0.1, causal)
+    for label, got in forms(gpu, q, k, v, news, lens, 0.1, causal):
         check_all(*got, want, label)
