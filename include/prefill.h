@@ -17,7 +17,8 @@
  * fp32 arithmetic of exact products; the softmax weights are rounded to bf16 for the
  * product with V and divided by the sum of the rounded ones; out is rounded to bf16.
  * A value that is not finite, an infinity as well, makes NaN of its dim in every row that
- * sees it. A query that is not finite makes NaN of its whole row.
+ * sees it. A query that is not finite makes NaN of its whole row, and so do keys whose
+ * scores are not finite, but for scores of -infinity beside a finite one (weight 0).
  * lse[row, h] is the natural logarithm of the sum of exp(scale * <q, K_j>).
  *
  * Rows without a place get zeros and an lse of -infinity: those of no request (before

@@ -816,6 +816,20 @@ __device__ __forceinline__ uint64_t keys_in_cache(const Args& a, const Work& w, 
   return __builtin_amdgcn_ballot_w64((uint32_t)id < (uint32_t)a.num_blocks);
 }
 
+// Whether the lane's row sees a key of this split at all, of one whose scores were all
+// -infinity if they were there. (The whole wave calls this.)
+__device__ __forceinline__ bool sees_keys(const Args& a, const Work& w, bool asked) {
+  const bool some = asked && w.seen > w.t0 * kKeys;
+  if (!w.strange || __builtin_amdgcn_ballot_w64(some) == 0) return some;
+  bool in_cache = false;
+  for (int tile = w.t0; tile < w.t1; ++tile) {
+    const uint64_t in = keys_in_cache(a, w, tile);
+    const int n = w.seen - tile * kKeys;
+    in_cache |= n > 0 && (in << (kKeys - min(max(n, 1), kKeys))) != 0;
+  }
+  return some && in_cache;
+}
+
 // The queries of the lane's row as matrix operands.
 __device__ __forceinline__ void load_queries(const Args& a, const Work& w, bf16x8_t (&q)[8]) {
   const uint16_t* src = a.q + (w.rows.first + w.token) * a.q_token_stride +
@@ -1005,14 +1019,20 @@ __global__ __launch_bounds__(64 * kWaves, 2) void prefill_kernel(Args a, int uni
     if (kWaves == 8 && !late) change_over();
   }
   st.l = xor32_sum(st.l);
-  if (w.t0 < w.t1) spoil(spoilt, w.seen, st);
+  if (w.t0 < w.t1) {
+    spoil(spoilt, w.seen, st);
+    // Keys, but scores of -infinity alone (infinite keys): 0 / 0. Another split may have others,
+    // so the split says so by a sum of 1 under a reference of -infinity.
+    if (sees_keys(a, w, st.m == kNegInf && st.l == 0.f)) st.l = a.splits > 1 ? 1.f : __builtin_nanf("");
+  }
   store_row(a, (w.rows.first + w.token) * a.Hq + w.head, w.split, st.m, st.l, st.o, w.valid);
 }
 
 // Joins the splits of a row, a wave each: a DPP row of 16 lanes takes every fourth split, 8
 // dims a lane, with a state of its own and the next two splits' loads in flight; the four
 // meet at the end, in the same order every time. (A split's (m, l) of (-infinity, 0) has no
-// keys; a NaN has an l of NaN, whatever its m.)
+// keys, of (-infinity, 1) scores of -infinity alone, which give NaN if no split has others; a
+// NaN has an l of NaN, whatever its m.)
 constexpr int kMergeWaves = 4;
 __global__ __launch_bounds__(64 * kMergeWaves) void prefill_merge_kernel(Args a) {
   const int row = (int)blockIdx.x * kMergeWaves +
@@ -1032,6 +1052,7 @@ __global__ __launch_bounds__(64 * kMergeWaves) void prefill_merge_kernel(Args a)
   };
   float m = kNegInf, l = 0.f;
   f32x4_t x[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+  bool hopeless = false;
   int s = lane >> 4;
   Piece next = load(s), after = load(s + 4);
   for (int s0 = 0; s0 < a.splits; s0 += 4, s += 4) {
@@ -1042,14 +1063,17 @@ __global__ __launch_bounds__(64 * kMergeWaves) void prefill_merge_kernel(Args a)
     const float top = fmaxf(m, now.ml.x), ref = top == kNegInf ? 0.f : top;
     const float old = m == kNegInf ? 0.f : exp2_fast(m - ref);
     const float f = now.ml.x == kNegInf ? 1.f : exp2_fast(now.ml.x - ref);
+    const bool all_infinite = now.ml.x == kNegInf && now.ml.y == 1.f;
+    hopeless |= all_infinite;
     m = top;
-    l = fmaf(l, old, now.ml.y * f);
+    l = fmaf(l, old, all_infinite ? 0.f : now.ml.y * f);
     x[0] = x[0] * old + now.v[0] * f;
     x[1] = x[1] * old + now.v[1] * f;
   }
   const float top = xor32_max(gqa::xor16_max(m));
   const float f = m == kNegInf ? (l == 0.f ? 0.f : 1.f) : exp2_fast(m - top);
-  const float sum = xor32_sum(gqa::xor16_sum(l * f));
+  float sum = xor32_sum(gqa::xor16_sum(l * f));
+  if (top == kNegInf && __builtin_amdgcn_ballot_w64(hopeless) != 0) sum = __builtin_nanf("");
   const float inv = sum == 0.f ? 0.f : 1.f / sum;
   float y[8];
 #pragma unroll

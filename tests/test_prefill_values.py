@@ -39,6 +39,12 @@ def forms(gpu, q, k, v, news, lens, scale, causal=True, splits=(1, 3), sizes=(16
                 cu_seqlens=tensor(cu_q, gpu), causal=causal, num_splits=ns, return_lse=True))
 
 
+def with_reach(want, of_finite):
+    """`want`, its tolerance being that of the keys with finite scores (those whose scores are
+    -infinity weigh nothing)."""
+    return want[:3] + (of_finite[3],) + want[4:]
+
+
 # Few rows behind many keys, prompts of some tiles of rows, and enough rows for eight waves.
 SHAPES = {
     "drafts": ([3, 1], [400, 90], 8, 2),
@@ -80,3 +86,67 @@ def test_infinite_values(gpu, shape, causal):
     want = packed_want(q, k, v, cu_q, cu_k, 0.1, causal)
     for label, got in forms(gpu, q, k, v, news, lens, 0.1, causal):
         check_all(*got, want, label)
+
+
+@pytest.mark.parametrize("shape", SHAPES)
+@pytest.mark.parametrize("scale", [0.1, -0.1])
+def test_infinite_keys(gpu, shape, scale):
+    """A key with an infinite score has no weight or gives NaN; a row whose keys' scores are all
+    -infinity gives NaN, in one split or all of them, and a row without keys zeros as ever."""
+    q, k, v, news, lens = rows(shape, 3)
+    news, at = news + [2, 1, 3, 2], sum(news)
+    Hq, Hkv, end = q.shape[1], k.shape[1], sum(lens)
+    gen = torch.Generator().manual_seed(4)
+    lens = lens + [2, 0, 200, 130]  # all infinite; no key; all infinite; the first 100 of 130
+    q = torch.cat([q, normal(gen, 8, Hq, D)])
+    k = torch.cat([k, normal(gen, 332, Hkv, D)])
+    v = torch.cat([v, normal(gen, 332, Hkv, D)])
+    q[:, :, 11] = q[:, :, 11].abs() + 1.0
+    k[5, 0, 11] = k[80, 1, 11] = k[end:end + 302, 0, 11] = -INF if scale > 0 else INF
+    k[20, 1, 11] = INF if scale > 0 else -INF  # (a score of +infinity: NaN)
+    cu_q, cu_k = sums(news), sums(lens)
+    for causal in (True, False):
+        finite = torch.where(torch.isfinite(k), k, 0.0)
+        want = with_reach(packed_want(q, k, v, cu_q, cu_k, scale, causal),
+                          packed_want(q, finite, v, cu_q, cu_k, scale, causal))
+        nan = np.isnan(want[0]).all(axis=2)
+        G = Hq // Hkv
+        assert nan[at:at + 2, :G].all() and not nan[at:at + 2, G:].any()
+        assert not want[0][at + 2].any() and nan[at + 3:at + 6, :G].all()
+        assert not nan[at + 6:, :].any()
+        for label, got in forms(gpu, q, k, v, news, lens, scale, causal, splits=(1, 2, 7)):
+            check_all(*got, want, label)
+
+
+def test_infinite_keys_and_ids_outside(gpu):
+    """Keys in blocks outside the cache are not seen: only the others' scores count."""
+    gen = torch.Generator().manual_seed(5)
+    Hq, Hkv, bs, lens, news = 4, 1, 16, [160, 160, 160], [3, 3, 3]
+    q, cu = normal(gen, 9, Hq, D), sums(news)
+    q[:, :, 0] = 1.0
+    table, num = pages(lens, bs, gen)
+    kc, vc = normal(gen, num, bs, Hkv, D), normal(gen, num, bs, Hkv, D)
+    kc[table[0].long()] = kc[table[1, :5].long()] = kc[table[2, 5:].long()] = 1.0
+    for ids in (table[0], table[1, :5], table[2, 5:]):
+        kc[ids.long(), :, :, 0] = -INF
+    table[0, 2:8] = -1   # what is left has scores of -infinity: NaN
+    table[1, 5:] = num   # as well
+    table[2, 5:] = -3    # finite ones are left
+    table[0, 0] = num + 5
+    finite = torch.where(torch.isfinite(kc), kc, 0.0)
+    want = with_reach(paged_want(q, kc, vc, table, lens, cu, 0.1, True),
+                      paged_want(q, finite, vc, table, lens, cu, 0.1, True))
+    assert np.isnan(want[0][:6]).all() and np.isfinite(want[0][6:]).all()
+    table4 = torch.cat([table, torch.full((1, 10), -1, dtype=torch.int32)])  # no key at all: zeros
+    cu4, q4 = sums(news + [2]), torch.cat([q, q[:2]])
+    want4 = with_reach(paged_want(q4, kc, vc, table4, lens + [100], cu4, 0.1, True),
+                       paged_want(q4, finite, vc, table4, lens + [100], cu4, 0.1, True))
+    for ns in (1, 2, 5):
+        check_all(*prefill.gqa_prefill(q.to(gpu), kc.to(gpu), vc.to(gpu), table.to(gpu),
+                                       tensor(lens, gpu), 0.1, cu_seqlens=tensor(cu, gpu),
+                                       num_splits=ns, return_lse=True), want, f"splits {ns}")
+        got = prefill.gqa_prefill(q4.to(gpu), kc.to(gpu), vc.to(gpu), table4.to(gpu),
+                                  tensor(lens + [100], gpu), 0.1, cu_seqlens=tensor(cu4, gpu),
+                                  num_splits=ns, return_lse=True)
+        check_all(*got, want4, f"splits {ns}, a request without keys")
+        assert not got[0][9:].any() and torch.isneginf(got[1][9:]).all()
