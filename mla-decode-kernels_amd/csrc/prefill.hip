@@ -408,7 +408,8 @@ constexpr float kSlack = 8.f;
 constexpr float kDown = 24.f;
 
 struct State {
-  float m, l;        // reference of the row's weights (a raw score), their sum in this half
+  float m;           // reference of the row's weights (a raw score)
+  float l, fine;     // their sums in this half: as they are multiplied, and in fp32
   f32x16_t o[4];     // o[d][i]: dim 32d + 8(i / 4) + 4h + i % 4
 };
 
@@ -490,10 +491,12 @@ __device__ __forceinline__ float reference(float m, float scale) {
 }
 
 // The weights of a tile as matrix operands, rounded to bf16 (off by 2^-8 of each at most);
-// their sum is taken of what is multiplied, so that rows of equal values come out exact.
+// their sum is taken of what is multiplied, so that rows of equal values come out exact. The
+// sum of the fp32 weights is taken where it is asked for, of exponentials of its own: 32 more
+// a lane and step, where sums kept in every call cost long prompts 2 %.
 template <int kBlocks>
-__device__ __forceinline__ void soften(const f32x16_t (&s)[kBlocks], float scale, State& st,
-                                       uint32_t (&p)[kBlocks * 8]) {
+__device__ __forceinline__ void soften(const f32x16_t (&s)[kBlocks], float scale, bool fine,
+                                       State& st, uint32_t (&p)[kBlocks * 8]) {
   float mx = s[0][0];
 #pragma unroll
   for (int b = 0; b < kBlocks; ++b)
@@ -509,6 +512,7 @@ __device__ __forceinline__ void soften(const f32x16_t (&s)[kBlocks], float scale
     st.m = m;
     if (!first) {  // (else there is nothing yet)
       st.l *= alpha;
+      st.fine *= alpha;
 #pragma unroll
       for (int d = 0; d < 4; ++d)
 #pragma unroll
@@ -516,6 +520,14 @@ __device__ __forceinline__ void soften(const f32x16_t (&s)[kBlocks], float scale
     }
   }
   const float ms = reference(st.m, scale);
+  if (fine) {
+    float sum = 0.f;
+#pragma unroll
+    for (int b = 0; b < kBlocks; ++b)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) sum += exp2_fast(fmaf(s[b][i], scale, -ms));
+    st.fine += sum;
+  }
   const bf16x2_t ones = {(__bf16)1.f, (__bf16)1.f};
 #pragma unroll
   for (int b = 0; b < kBlocks; ++b)
@@ -658,12 +670,22 @@ __device__ __forceinline__ void spoil(const Spoilt& spoilt, int seen, State& st)
 // whose tile the row sees whole: they were multiplied, and infinities may have stayed such.
 __device__ __forceinline__ float number(float x) { return fmaf(x, 0.f, x); }
 
-// A row's result: to out and lse, or to the states of split `split`.
-__device__ __forceinline__ void store_row(const Args& a, int row, int split, float m, float l,
-                                          const f32x16_t (&o)[4], bool valid) {
+// The natural logarithm of a sum of weights held against `ref` (2^-kDown of the usual).
+__device__ __forceinline__ float log_sum(float ref, float sum) {
+  return sum == 0.f ? kNegInf : ((ref - kDown) + __log2f(sum * (float)(1 << (int)kDown))) * gqa::kLn2;
+}
+
+// A row's result: to out and lse, or to the states of split `split`. A split's sums of values
+// are brought from the rounded weights' sum to the fp32 weights', by which the splits are
+// weighed against each other.
+__device__ __forceinline__ void store_row(const Args& a, int row, int split, const State& st,
+                                          bool valid) {
   const int h = (threadIdx.x >> 5) & 1;
+  const float m = st.m, l = st.l;
+  const f32x16_t(&o)[4] = st.o;
   if (a.splits > 1) {
     if (!valid) return;
+    const float f = st.fine / l;
     const size_t at = (size_t)row * a.splits + split;
     float* dst = a.states + at * kDim;
     if (!(m == kNegInf && l == 0.f))  // (else nobody reads it)
@@ -672,8 +694,8 @@ __device__ __forceinline__ void store_row(const Args& a, int row, int split, flo
 #pragma unroll
       for (int i = 0; i < 16; i += 4)
         *reinterpret_cast<f32x4_t*>(dst + 32 * d + 2 * i + 4 * h) =
-            f32x4_t{o[d][i], o[d][i + 1], o[d][i + 2], o[d][i + 3]};
-    if (h == 0) a.sums[at] = make_float2(m == kNegInf ? kNegInf : reference(m, a.scale), l);
+            f32x4_t{o[d][i] * f, o[d][i + 1] * f, o[d][i + 2] * f, o[d][i + 3] * f};
+    if (h == 0) a.sums[at] = make_float2(m == kNegInf ? kNegInf : reference(m, a.scale), st.fine);
     return;
   }
   const float inv = l == 0.f ? 0.f : 1.f / l;
@@ -695,8 +717,7 @@ __device__ __forceinline__ void store_row(const Args& a, int row, int split, flo
         *reinterpret_cast<u32x4_t*>(dst + 32 * d + 2 * i + 8 * h) =
             u32x4_t{p0[0], p1[0], p0[1], p1[1]};
     }
-  if (a.lse && valid && h == 0)
-    a.lse[row] = l == 0.f ? kNegInf : (reference(m, a.scale) + __log2f(l)) * gqa::kLn2;
+  if (a.lse && valid && h == 0) a.lse[row] = log_sum(reference(m, a.scale), st.fine);
 }
 
 // The arguments that a workgroup's start needs, in registers from here on: the compiler loads
@@ -718,7 +739,7 @@ __device__ __forceinline__ void fetch(const Args& a, int units) {
     asm volatile("" : : "s"(a.block_bytes32), "s"(a.token_bytes32), "s"(a.tile_blocks),
                  "s"(a.tile_slots));
   asm volatile("" : : "s"(a.q), "s"(a.q_token_stride), "s"(a.q_head_stride), "s"(a.flip),
-               "s"(a.scale));
+               "s"(a.scale), "s"(a.lse), "s"(a.splits));
   fetch(a.head_div);
   fetch(a.group_div);
   if constexpr (kSource != kPacked) fetch(a.bs_div);
@@ -863,7 +884,7 @@ __device__ __forceinline__ void settle_queries(bf16x8_t (&q)[8], uint32_t flip) 
 
 __device__ __forceinline__ void clear(State& st) {
   st.m = kNegInf;
-  st.l = 0.f;
+  st.l = st.fine = 0.f;
 #pragma unroll
   for (int d = 0; d < 4; ++d)
 #pragma unroll
@@ -929,6 +950,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void prefill_kernel(Args a, int uni
 
   State st;
   clear(st);
+  const bool fine = a.lse != nullptr || a.splits > 1;
   if (w.t0 < w.t1) {
     feed.begin(a, w.keys, w.t0, wave * kRun, lane);
     copy_keys(w.t0);
@@ -974,8 +996,9 @@ __global__ __launch_bounds__(64 * kWaves, 2) void prefill_kernel(Args a, int uni
       constexpr uint32_t kNext = (decltype(slot)::value + 1) % kSlots * kSlotBytes;
       refill(tile);
       uint32_t p[16];
-      soften<2>(s, a.scale, st, p);
+      soften<2>(s, a.scale, fine, st, p);
       settle(st.l);
+      settle(st.fine);
 #pragma unroll
       for (int i = 0; i < 16; ++i) settle(p[i]);
       if constexpr (kWaves == 8) change_over();
@@ -997,8 +1020,9 @@ __global__ __launch_bounds__(64 * kWaves, 2) void prefill_kernel(Args a, int uni
       refill(tile);
       uint32_t p[16];
       take_out<2>(s, w.seen - tile * kKeys, keys_in_cache(a, w, tile));
-      soften<2>(s, a.scale, st, p);
+      soften<2>(s, a.scale, fine, st, p);
       settle(st.l);
+      settle(st.fine);
 #pragma unroll
       for (int i = 0; i < 16; ++i) settle(p[i]);
       if constexpr (kWaves == 8) change_over();
@@ -1019,13 +1043,15 @@ __global__ __launch_bounds__(64 * kWaves, 2) void prefill_kernel(Args a, int uni
     if (kWaves == 8 && !late) change_over();
   }
   st.l = xor32_sum(st.l);
+  st.fine = xor32_sum(st.fine);
   if (w.t0 < w.t1) {
     spoil(spoilt, w.seen, st);
     // Keys, but scores of -infinity alone (infinite keys): 0 / 0. Another split may have others,
     // so the split says so by a sum of 1 under a reference of -infinity.
-    if (sees_keys(a, w, st.m == kNegInf && st.l == 0.f)) st.l = a.splits > 1 ? 1.f : __builtin_nanf("");
+    if (sees_keys(a, w, st.m == kNegInf && st.l == 0.f))
+      st.l = st.fine = a.splits > 1 ? 1.f : __builtin_nanf("");
   }
-  store_row(a, (w.rows.first + w.token) * a.Hq + w.head, w.split, st.m, st.l, st.o, w.valid);
+  store_row(a, (w.rows.first + w.token) * a.Hq + w.head, w.split, st, w.valid);
 }
 
 // Joins the splits of a row, a wave each: a DPP row of 16 lanes takes every fourth split, 8
@@ -1081,7 +1107,7 @@ __global__ __launch_bounds__(64 * kMergeWaves) void prefill_merge_kernel(Args a)
   if (lane < 16)
     reinterpret_cast<u32x4_t*>(a.out + (size_t)row * kDim)[i] =
         u32x4_t{pack2(y[0], y[1]), pack2(y[2], y[3]), pack2(y[4], y[5]), pack2(y[6], y[7])};
-  if (a.lse && lane == 0) a.lse[row] = sum == 0.f ? kNegInf : (top + __log2f(sum)) * gqa::kLn2;
+  if (a.lse && lane == 0) a.lse[row] = log_sum(top, sum);
 }
 
 // ---------------------------------------------------------------------------- host

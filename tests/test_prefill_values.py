@@ -150,3 +150,31 @@ def test_infinite_keys_and_ids_outside(gpu):
                                   num_splits=ns, return_lse=True)
         check_all(*got, want4, f"splits {ns}, a request without keys")
         assert not got[0][9:].any() and torch.isneginf(got[1][9:]).all()
+
+
+@pytest.mark.parametrize("shape", SHAPES)
+def test_log_sums_are_of_fp32_weights(gpu, shape):
+    """The log-sum-exps of few large weights, which bf16 would move by up to 2^-8. Of 4 dims: their
+    raw scores are off by 4 * 2^-24 of the sum of |q k|, 3 roundings more until the exponent,
+    which the tolerance doubles; the exponential 2^-22, twice for a sum that is rescaled; sums
+    of 64 keys in a row, one of them to the next; the logarithm and its sum with the
+    reference, 4 steps of fp32 of the result and 2^-20."""
+    q, k, v, news, lens = rows(shape, 6)
+    q[:, :, 4:], k[:, :, 4:] = 0.0, 0.0
+    scale = 2.0
+    cu_q, cu_k = sums(news), sums(lens)
+    for causal in (True, False):
+        want = packed_want(q, k, v, cu_q, cu_k, scale, causal)
+        _, want_lse, _, reach, count = want
+        tol = (16 * 2.0 ** -24 * reach + 2.0 ** -21 + (count / 64 + 64) * 2.0 ** -24
+               + 4 * 2.0 ** -23 * np.abs(want_lse) + 2.0 ** -20)
+        plain = {}
+        for label, (out, lse) in forms(gpu, q, k, v, news, lens, scale, causal):
+            check_all(out, lse, want, label)
+            off = np.abs(f64(lse) - want_lse) / tol
+            assert (off <= 1).all(), f"{label}: lse off by {off.max()} of the tolerance"
+            plain[label] = out
+        for ns in (1, 3):  # and the results are the same without them
+            got = prefill.gqa_prefill_packed(q.to(gpu), k.to(gpu), v.to(gpu), tensor(cu_q, gpu),
+                                             tensor(cu_k, gpu), scale, causal=causal, num_splits=ns)
+            assert torch.equal(got, plain[f"rows, splits {ns}"])
