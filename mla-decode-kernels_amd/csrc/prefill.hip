@@ -492,11 +492,13 @@ __device__ __forceinline__ float reference(float m, float scale) {
 
 // The weights of a tile as matrix operands, rounded to bf16 (off by 2^-8 of each at most);
 // their sum is taken of what is multiplied, so that rows of equal values come out exact. The
-// sum of the fp32 weights is taken where it is asked for, of exponentials of its own: 32 more
-// a lane and step, where sums kept in every call cost long prompts 2 %.
-template <int kBlocks>
-__device__ __forceinline__ void soften(const f32x16_t (&s)[kBlocks], float scale, bool fine,
-                                       State& st, uint32_t (&p)[kBlocks * 8]) {
+// sum of the fp32 weights, for log-sum-exps and splits, is taken beside it with kFine, which
+// the loop over whole tiles has a form of its own for: 32 additions a lane and step cost a
+// prompt of 16384 tokens 2 % and a branch around them 4 chunks 2 %. (The few tiles that are
+// seen in part have them always.)
+template <int kBlocks, bool kFine>
+__device__ __forceinline__ void soften(const f32x16_t (&s)[kBlocks], float scale, State& st,
+                                       uint32_t (&p)[kBlocks * 8]) {
   float mx = s[0][0];
 #pragma unroll
   for (int b = 0; b < kBlocks; ++b)
@@ -512,7 +514,7 @@ __device__ __forceinline__ void soften(const f32x16_t (&s)[kBlocks], float scale
     st.m = m;
     if (!first) {  // (else there is nothing yet)
       st.l *= alpha;
-      st.fine *= alpha;
+      if constexpr (kFine) st.fine *= alpha;
 #pragma unroll
       for (int d = 0; d < 4; ++d)
 #pragma unroll
@@ -520,24 +522,20 @@ __device__ __forceinline__ void soften(const f32x16_t (&s)[kBlocks], float scale
     }
   }
   const float ms = reference(st.m, scale);
-  if (fine) {
-    float sum = 0.f;
-#pragma unroll
-    for (int b = 0; b < kBlocks; ++b)
-#pragma unroll
-      for (int i = 0; i < 16; ++i) sum += exp2_fast(fmaf(s[b][i], scale, -ms));
-    st.fine += sum;
-  }
+  float sum = 0.f;
   const bf16x2_t ones = {(__bf16)1.f, (__bf16)1.f};
 #pragma unroll
   for (int b = 0; b < kBlocks; ++b)
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      p[8 * b + i] = pack2(exp2_fast(fmaf(s[b][2 * i], scale, -ms)),
-                           exp2_fast(fmaf(s[b][2 * i + 1], scale, -ms)));
+      const float x = exp2_fast(fmaf(s[b][2 * i], scale, -ms));
+      const float y = exp2_fast(fmaf(s[b][2 * i + 1], scale, -ms));
+      if constexpr (kFine) sum += x + y;
+      p[8 * b + i] = pack2(x, y);
       st.l = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2_t, p[8 * b + i]), ones, st.l,
                                              false);
     }
+  if constexpr (kFine) st.fine += sum;
 }
 
 template <int kWords>
@@ -991,14 +989,13 @@ __global__ __launch_bounds__(64 * kWaves, 2) void prefill_kernel(Args a, int uni
       meet();
     };
     // A step whose tile all rows see; the tile is in slot kSlot.
-    const auto step = [&](auto slot) __attribute__((always_inline)) {
+    const auto step = [&](auto slot, auto sum) __attribute__((always_inline)) {
       constexpr uint32_t kHere = decltype(slot)::value * kSlotBytes;
       constexpr uint32_t kNext = (decltype(slot)::value + 1) % kSlots * kSlotBytes;
       refill(tile);
       uint32_t p[16];
-      soften<2>(s, a.scale, fine, st, p);
+      soften<2, decltype(sum)::value>(s, a.scale, st, p);
       settle(st.l);
-      settle(st.fine);
 #pragma unroll
       for (int i = 0; i < 16; ++i) settle(p[i]);
       if constexpr (kWaves == 8) change_over();
@@ -1007,20 +1004,26 @@ __global__ __launch_bounds__(64 * kWaves, 2) void prefill_kernel(Args a, int uni
       arrive(tile);
       return ++tile < w.full;
     };
-    while (tile < w.full) {
-      if (!step(std::integral_constant<int, 0>{})) break;
-      if (!step(std::integral_constant<int, 1>{})) break;
-      if constexpr (kSlots == 4) {
-        if (!step(std::integral_constant<int, 2>{})) break;
-        if (!step(std::integral_constant<int, 3>{})) break;
+    const auto steps = [&](auto sum) __attribute__((always_inline)) {
+      while (tile < w.full) {
+        if (!step(std::integral_constant<int, 0>{}, sum)) break;
+        if (!step(std::integral_constant<int, 1>{}, sum)) break;
+        if constexpr (kSlots == 4) {
+          if (!step(std::integral_constant<int, 2>{}, sum)) break;
+          if (!step(std::integral_constant<int, 3>{}, sum)) break;
+        }
       }
-    }
+    };
+    if (fine)
+      steps(std::true_type{});
+    else
+      steps(std::false_type{});
     // Tiles that some rows see in part; behind the last one are no scores to take.
     const auto part_step = [&](auto last) __attribute__((always_inline)) {
       refill(tile);
       uint32_t p[16];
       take_out<2>(s, w.seen - tile * kKeys, keys_in_cache(a, w, tile));
-      soften<2>(s, a.scale, fine, st, p);
+      soften<2, true>(s, a.scale, st, p);
       settle(st.l);
       settle(st.fine);
 #pragma unroll
