@@ -38,7 +38,10 @@ extern "C" {
  * grows the older tokens' codes are rounded again under the new scale. Slots behind the
  * new tokens stay as they are. A code is the nearest one, ties to even; infinities and
  * NaN are held as NaN.
- *   A scale thus only grows while a tile fills, and is set anew by a token in slot 0. */
+ *   A scale thus only grows while a tile fills, and is set anew by a token in slot 0.
+ *   Sizes whose launch would have 2^32 threads or more are refused (256 for each kv-head
+ * of T / 16 + 2 B tiles, or of T without cu_seqlens, a quarter of that for the values, and
+ * 256 for 4 tokens and 16 heads of the queries). */
 GQA_DECODE_API int kv8_append_launch(const kv_append_args* args, uint8_t* codes, uint8_t* scales,
                                      hipStream_t stream);
 

@@ -80,6 +80,8 @@ typedef struct prefill_gqa_args {
 /* num_splits > 0: every request's keys are cut into that many pieces, whose partial
  * results a second launch joins in order (1: no second launch). 0: chosen from the
  * sizes and the current device's CU count; the host never reads the lengths.
+ * Sizes whose launches would have 2^32 threads or more are refused: none with T Hq / 128 +
+ * (B + 2) Hkv below 2^23 and, where there is a second launch, T Hq up to 2^26 - 4.
  * workspace: prefill_gqa_workspace_bytes(args, num_splits) bytes (it may be 0), 16-byte
  * aligned, uninitialised; launches that share one must not overlap. */
 GQA_DECODE_API int prefill_gqa_launch(const prefill_gqa_args* args, int num_splits,

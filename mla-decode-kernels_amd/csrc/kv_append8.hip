@@ -441,7 +441,7 @@ extern "C" int kv8_append_launch(const kv_append_args* args, uint8_t* codes, uin
   g.group_div = make_fastdiv(g.q_groups);
   const int64_t k_blocks = units * a.Hkv, v_blocks = (k_blocks + kWaves - 1) / kWaves;
   const int64_t blocks = k_blocks + v_blocks + groups * g.q_groups;
-  if (blocks > INT32_MAX) return hipErrorInvalidValue;
+  if (blocks * 64 * kWaves > UINT32_MAX) return hipErrorInvalidValue;  // (threads of a launch)
   g.k_blocks = (unsigned)k_blocks;
   g.v_blocks = (unsigned)v_blocks;
   if (R == 1)

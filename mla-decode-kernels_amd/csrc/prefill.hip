@@ -1181,11 +1181,17 @@ size_t states_bytes(const prefill_gqa_args& p, int splits) {
   return splits > 1 ? (size_t)p.T * p.Hq * splits * (kDim * sizeof(float) + sizeof(float2)) : 0;
 }
 
+// A launch has fewer than 2^32 threads in a dimension.
+bool launches_fit(const prefill_gqa_args& p, const Plan& plan) {
+  const int64_t most = UINT32_MAX, rows = (int64_t)p.T * p.Hq;
+  if (units_of(p, kRows * plan.waves) * p.Hkv * 64 * plan.waves > most) return false;
+  return plan.splits == 1 || (rows + kMergeWaves - 1) / kMergeWaves * 64 * kMergeWaves <= most;
+}
+
 using Kernel = void (*)(Args, int);
 
 hipError_t launch(const Args& a, const prefill_gqa_args& p, int waves, hipStream_t stream) {
   const int64_t units = units_of(p, kRows * waves);
-  if (units * p.Hkv > INT32_MAX) return hipErrorInvalidValue;
   // A prompt of 4096 tokens, 32Q/8KV: 133 us in blocks of 16 or 24, 223 in blocks of 12 and
   // 235 in blocks of 15, whose ids are found row by row.
   const int source = p.cu_seqlens_k                        ? kPacked
@@ -1242,6 +1248,7 @@ extern "C" int prefill_gqa_launch(const prefill_gqa_args* args, int num_splits, 
     return hipErrorInvalidValue;
   if (!packed && p.B > 0 && (!p.block_table || !p.seq_lens)) return hipErrorInvalidValue;
   const Plan plan = plan_of(p, num_splits);
+  if (!launches_fit(p, plan)) return hipErrorInvalidValue;
   const size_t need = states_bytes(p, plan.splits);
   if (need > 0 && (!workspace || misaligned(workspace, 16) || workspace_bytes < need))
     return hipErrorInvalidValue;
