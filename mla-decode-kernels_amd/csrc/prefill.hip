@@ -404,8 +404,9 @@ struct Feed {
 
 constexpr float kSlack = 8.f;
 // Weights are 2^-kDown of the usual, so that sums of 2^24 weighted values of any magnitude
-// stay in fp32's range. (What is lost for it are weights below 2^-102 of the largest.)
-constexpr float kDown = 24.f;
+// stay in fp32's range, by kSlack as well. (What is lost for it are weights below 2^-94 of
+// the reference's.)
+constexpr float kDown = 32.f, kUp = 0x1p32f;
 
 struct State {
   float m;           // reference of the row's weights (a raw score)
@@ -670,7 +671,7 @@ __device__ __forceinline__ float number(float x) { return fmaf(x, 0.f, x); }
 
 // The natural logarithm of a sum of weights held against `ref` (2^-kDown of the usual).
 __device__ __forceinline__ float log_sum(float ref, float sum) {
-  return sum == 0.f ? kNegInf : ((ref - kDown) + __log2f(sum * (float)(1 << (int)kDown))) * gqa::kLn2;
+  return sum == 0.f ? kNegInf : ((ref - kDown) + __log2f(sum * kUp)) * gqa::kLn2;
 }
 
 // A row's result: to out and lse, or to the states of split `split`. A split's sums of values
