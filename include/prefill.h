@@ -19,7 +19,7 @@
  * A value that is not finite, an infinity as well, makes NaN of its dim in every row that
  * sees it. A query that is not finite makes NaN of its whole row, and so do keys whose
  * scores are not finite, but for scores of -infinity beside a finite one (weight 0).
- * lse[row, h] is the natural logarithm of the sum of exp(scale * <q, K_j>).
+ * lse[row, h] is the natural logarithm of the sum of exp(scale * <q, K_j>), in fp32.
  *
  * Rows without a place get zeros and an lse of -infinity: those of no request (before
  * cu_seqlens_q[0], from cu_seqlens_q[B] on) and those at a negative position (L < n).
@@ -78,8 +78,9 @@ typedef struct prefill_gqa_args {
 } prefill_gqa_args;
 
 /* num_splits > 0: every request's keys are cut into that many pieces, whose partial
- * results a second launch joins in order (1: no second launch). 0: chosen from the
- * sizes and the current device's CU count; the host never reads the lengths.
+ * results a second launch joins in order (1: no second launch). Paged pieces are equal
+ * parts of max_blocks * block_size tokens, whatever of them a request has. 0: chosen from
+ * the sizes and the current device's CU count; the host never reads the lengths.
  * Sizes whose launches would have 2^32 threads or more are refused: none with T Hq / 128 +
  * (B + 2) Hkv below 2^23 and, where there is a second launch, T Hq up to 2^26 - 4.
  * workspace: prefill_gqa_workspace_bytes(args, num_splits) bytes (it may be 0), 16-byte

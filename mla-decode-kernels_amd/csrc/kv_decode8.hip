@@ -10,9 +10,9 @@
 //   What bounds it: HBM, at 256 bytes a token and kv-head. 32 requests of 8192 tokens
 // (32Q/8KV, blocks of 16: 537 MB) take 86 us, merge launch and all (6.2 TB/s); 64 ragged
 // ones up to 32768 (64Q/8KV: 2.1 GB) 331 us (6.5 TB/s); 128 of 777 (205 MB) 38 us (5.4
-// TB/s). One request of 512 tokens takes 7.3 us, two launches and their loads in a row. When
-// a workgroup keeps whole segments is decided as for the 4-bit cache: the rule was looked
-// over at these sizes and holds.
+// TB/s). One request of 512 tokens takes 7.3 us, one launch whose loads wait for each other.
+// When a workgroup keeps whole segments is decided as for the 4-bit cache: the rule was
+// looked over at these sizes and holds.
 #include "kv_cache8.h"
 #include "kv_common8.hpp"
 #include "kv_decode_scan.hpp"

@@ -22,7 +22,13 @@
 // is moved (and sums rescaled) only where a tile exceeds it by 2^8, so that the sums stay
 // in fp32's range and most steps rescale nothing. The weights enter the second product
 // as bf16 (off by up to 2^-8 of themselves each); the sum they are divided by is of the
-// rounded weights, in fp32, so that an equal error of all of them cancels.
+// rounded weights, in fp32, so that an equal error of all of them cancels. Log-sum-exps, and
+// what splits weigh against each other, are of the fp32 weights.
+//   Weights of two bf16 parts (off by 2^-16) take 16 matrix instructions more a step: a
+// prompt of 16384 tokens 2756 us for 1876, 13 prompts and chunks 568 for 401, 32 packed prompts
+// 262 for 213, one of 100 tokens 8.9 for 8.2; a request's drafts 3 to 38 % (5 and 30 of them
+// behind 32000 keys), where a step's products are not hidden. All forms round alike, so that
+// a request's rows come out the same whatever else is in the call (in the same splits).
 //
 // Tiles of 64 keys: 32 matrix instructions a wave and step, 1024 cycles of a SIMD, on
 // 32 KB read from LDS. 8 waves, two to a SIMD, share a tile and run half a step apart, so
@@ -32,16 +38,16 @@
 // LDS per product.
 //   What bounds it:
 //   - a long prompt: the matrix rate and LDS. 16384 tokens (32Q/8KV, causal, 2199 GFLOP)
-//     take 1.80-1.86 ms, 1.18-1.22 PFLOP/s; a library product of 8192^3 reaches 1.29 on the
+//     take 1.80-1.91 ms, 1.15-1.22 PFLOP/s; a library product of 8192^3 reaches 1.29 on the
 //     same card. The matrix units are busy 62 % of the cycles, at some 1.8 GHz, and LDS some
 //     70 %: 32 rows a wave read 128 bytes a cycle and CU for products at full rate, which is
 //     all it gives. (64 rows a wave would read half, on 512 registers and one wave a SIMD,
 //     whose softmax would have to go between its own products.)
-//   - prompts of some 500 tokens (64Q/8KV, 32 of them, packed: 213 us, 0.61 PFLOP/s): starts
+//   - prompts of some 500 tokens (64Q/8KV, 32 of them, packed: 209-217 us, 0.6 PFLOP/s): starts
 //     and ends of workgroups 5 tiles long (of some 29000 cycles 15000 are in the loop).
-//   - drafts over long caches: HBM (16 requests, 454 MB: 98 us, 4.6 TB/s, the merge of the
+//   - drafts over long caches: HBM (16 requests, 454 MB: 93-105 us, 4.6 TB/s, the merge of the
 //     splits with it).
-//   - a prompt of 100 tokens (8.2 us): the chain of its loads.
+//   - a prompt of 100 tokens (8.4 us): the chain of its loads.
 #include <math.h>
 
 #include <algorithm>
@@ -1293,7 +1299,9 @@ extern "C" int prefill_gqa_launch(const prefill_gqa_args* args, int num_splits, 
   a.flip = p.scale < 0.f ? 0x80008000u : 0u;
   // 4 chunks of up to 1024 rows over up to 8000 keys (with 30 us of read-back) 220 us, in the
   // requests' own order 221 to 265. One request, or one workgroup a request, has nothing to
-  // put in order, and for more requests looking through all of them costs more than it gives.
+  // put in order, and for more requests looking through all of them costs prompts more than it
+  // gives: in order and not, 17 prompts 16, 17 us (up to 200 tokens) and 89, 86 (1000), 32 139,
+  // 122 (1000), 62 37, 24 (100), where 62 chunks of up to 100 behind up to 3000 take 116, 142.
   a.sorted = p.B >= 2 && p.B <= 16 && (int64_t)p.T * a.G > (int64_t)kRows * plan.waves * p.B;
   a.group_div = make_fastdiv((uint32_t)a.G);
   a.head_div = make_fastdiv((uint32_t)p.Hkv);

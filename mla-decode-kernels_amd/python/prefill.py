@@ -27,8 +27,15 @@ logarithms of the softmax sums, fp32 [T, Hq], from which results over parts of t
 can be joined. Rows without a place (of no request, or at a negative position) and
 rows that see no key get zeros and -infinity. Block ids outside the cache are left out.
 
+The softmax weights are rounded to bf16 (by 2^-8 of each at most) for the product with the
+values and divided by the sum of the rounded ones; log-sum-exps are of the fp32 weights.
+Values, queries and scores that are not finite give NaN to the rows that see them (a value
+in its dim alone), but for scores of -infinity beside finite ones, which weigh nothing.
+
 num_splits > 0 cuts every request's keys into so many pieces and joins them in a
-second launch; 0 chooses from the sizes (block_table's width among them). The
+second launch; 0 chooses from the sizes. Over paged caches the pieces are of what
+block_table's width holds: a table much wider than the longest request leaves most of
+them empty and few workgroups with the work (pass the columns in use, or more pieces). The
 operators run on the current stream, allocate their results (and a workspace)
 from torch's allocator and can be captured into graphs. Rejected arguments raise
 RuntimeError. There is no fallback: a missing build raises ImportError.
