@@ -1211,8 +1211,10 @@ hipError_t launch(const Args& a, const prefill_gqa_args& p, int waves, hipStream
        prefill_kernel<4, kPacked, true>},
       {prefill_kernel<8, kPaged, false>, prefill_kernel<8, kGather, false>,
        prefill_kernel<8, kPacked, false>}};
-  // Rows of one workgroup a request: nobody else reads its keys. (Drafts, 16 requests of up
-  // to 5 rows behind up to 16000 keys, 64Q/8KV, 454 MB: 107 us with nt, 119 without.)
+  // Rows of one workgroup a request, on average: nobody else reads most of the keys. (Drafts, 16
+  // requests of up to 5 rows behind up to 16000 keys, 64Q/8KV, 454 MB: 107 us with nt, 119
+  // without; 60 single rows behind up to 4000 keys, 32Q/8KV, 114, 126; with a chunk of 512
+  // rows behind 8000 among them 197, 201, of 1500 behind 16000 560, 522.)
   const bool once = (int64_t)p.T * a.G <= (int64_t)kRows * waves * p.B;
   const Kernel kernel = kernels[waves == 8 ? 2 : once][source];
   const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel),
