@@ -26,9 +26,9 @@
 // what splits weigh against each other, are of the fp32 weights.
 //   Weights of two bf16 parts (off by 2^-16) take 16 matrix instructions more a step: a
 // prompt of 16384 tokens 2756 us for 1876, 13 prompts and chunks 568 for 401, 32 packed prompts
-// 262 for 213, one of 100 tokens 8.9 for 8.2; a request's drafts 3 to 38 % (5 and 30 of them
-// behind 32000 keys), where a step's products are not hidden. All forms round alike, so that
-// a request's rows come out the same whatever else is in the call (in the same splits).
+// 262 for 213, one of 100 tokens 8.9 for 8.2; a request's 5 drafts behind 32000 keys 38 for 36
+// and 30 of them 62 for 45, where nothing hides a step's products. All forms round alike, so
+// that a request's rows come out the same whatever else is in the call (in the same splits).
 //
 // Tiles of 64 keys: 32 matrix instructions a wave and step, 1024 cycles of a SIMD, on
 // 32 KB read from LDS. 8 waves, two to a SIMD, share a tile and run half a step apart, so
